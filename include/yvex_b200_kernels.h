@@ -438,6 +438,106 @@ int yvex_b200_attention_f32(const float *q, const float *keys, const float *valu
 int yvex_b200_attention_sink(const float *query, const float *rows, const float *sinks, uint64_t heads, uint64_t row_count,
                              uint64_t head_dim, double scale, int round_bf16, float *out, int *status, void *stream);
 
+/*
+ * A serving step over a paged cache: four entries that share one description of the step. None has a counterpart
+ * in the reference, whose attention op reads one contiguous session (src/backend/cpu.c:319-411).
+ *
+ * The cache: k and v are [pages][kv_heads][page_size][head_dim] of F16 (qtype 1) or BF16 (30), 16-byte aligned;
+ * page_size is a multiple of 16, head_dim 64, 128 or 256. A cache of whole sessions [sessions][kv_heads][context][head_dim],
+ * as yvex_b200_attention_gqa_decode reads it, is the case of one page per session.
+ *
+ * The step: request r has cached[r] tokens in its pages already and brings fresh[r] more (one, a drafted chain or
+ * tree, a chunk of a prompt). Its token n lies in page block_table[r * table_width + n / page_size]. The fresh tokens
+ * of all requests are packed rows: those of r are offsets[r] .. offsets[r + 1] - 1. `tokens` is the number of rows the
+ * arrays have room for; rows from offsets[requests] on are padding (a captured graph's batch may be larger than the
+ * step). longest_fresh and longest bound fresh[r] and cached[r] + fresh[r]; they choose and size launches, the
+ * lengths themselves stay on the device. tree: parents[row] is the index of the row's parent among its request's
+ * fresh tokens, below the row's own, or -1 for a child of the last cached token; a tree has at most
+ * YVEX_B200_TREE_NODES nodes and ancestors[row] has the bits of the nodes that the row sees, its own among them.
+ * Without tree the fresh tokens are a chain: each sees those before it and itself. All lengths, ids and tables are int32
+ * device arrays.
+ */
+#define YVEX_B200_TREE_NODES 64
+typedef struct yvex_b200_kv_cache {
+    unsigned int qtype;
+    uint64_t pages, page_size, kv_heads, head_dim;
+    void *k, *v;
+} yvex_b200_kv_cache;
+typedef struct yvex_b200_kv_step {
+    uint64_t requests, tokens, table_width, longest_fresh, longest;
+    int tree;
+    const int32_t *cached, *fresh, *parents;
+    int32_t *block_table, *offsets;     /* [requests x table_width], [requests + 1] */
+    int64_t *slots;                     /* [tokens] page * page_size + place in the page; -1: none */
+    int32_t *positions, *row_request;   /* [tokens] */
+    uint64_t *ancestors;                /* [tokens], trees only */
+} yvex_b200_kv_step;
+
+/*
+ * Plans a step on the device from cached, fresh (and parents): offsets, slots, positions (cached + index in a chain,
+ * cached + depth in a tree), row_request and ancestors are written; requests that grow past their last page get pages
+ * free_pages[0..], in order of request and page, which are entered in block_table; *pages_used (device) is how many.
+ * Entries of block_table below ceil(cached / page_size) are read, others are left alone. Padding rows get slot and
+ * request -1, position and mask 0. Of `cache` only pages and page_size are read. Status 2: a negative length, one above its bound, more rows
+ * than `tokens`, more pages than free_count or table_width, a page id outside the cache, a parent not below its
+ * child: the rows concerned get slot -1 (a bad parent counts as -1), the others are planned.
+ */
+int yvex_b200_kv_plan(const yvex_b200_kv_cache *cache, const yvex_b200_kv_step *step, const int32_t *free_pages,
+                      uint64_t free_count, int32_t *pages_used, int *status, void *stream);
+/*
+ * Stores row t of k and v ([tokens][kv_heads][head_dim] of F32, F16 or BF16; token strides in elements; 16-byte aligned
+ * rows) at slots[t] of the cache, rounded to nearest even; negative slots are skipped. `slots` are those of the step,
+ * or others: rows of the accepted path of a tree are stored again behind the cached tokens that way. The
+ * slots of one call are distinct. Status 1: a value that is not finite after rounding (stored all the same); 2: a slot past the cache (not stored).
+ */
+int yvex_b200_kv_append(const yvex_b200_kv_cache *cache, const int64_t *slots, uint64_t tokens, unsigned int qtype,
+                        const void *k, uint64_t k_stride, const void *v, uint64_t v_stride, int *status, void *stream);
+/*
+ * Attention of the fresh tokens over the pages, their own rows among them (append comes first): q [tokens] rows of
+ * [q_heads][head_dim] in the cache's type (q_stride: elements between rows, 16-byte aligned), out packed alike in the
+ * cache's type, f32 scores, softmax and sums. Query heads share kv heads in groups of q_heads / kv_heads. A row that
+ * sees no key (an empty mask over an empty cache) is zero; padding rows of out are left as they were. Keys that a row does
+ * not see have no influence on it, whatever is stored there. Of the step's arrays cached, block_table, offsets and ancestors
+ * (trees) are read. Status 1: an output that is not finite; 2: lengths above their bounds, offsets that are not those of a
+ * plan, a page id outside the cache (its keys then count as unseen). workspace: yvex_b200_attention_paged_workspace_bytes of the same cache
+ * and step bounds, 16-byte aligned; calls that may overlap in time need one each.
+ */
+uint64_t yvex_b200_attention_paged_workspace_bytes(const yvex_b200_kv_cache *cache, const yvex_b200_kv_step *step, uint64_t q_heads);
+int yvex_b200_attention_paged(const yvex_b200_kv_cache *cache, const yvex_b200_kv_step *step, const void *q, uint64_t q_stride,
+                              uint64_t q_heads, float scale, void *out, void *workspace, uint64_t workspace_bytes,
+                              int *status, void *stream);
+
+/*
+ * Edits of the output head's rows before a token is chosen. For row t of request r and word w:
+ *   x = logits[t][w]; where w occurs in r's history or on t's drafted path: x = x > 0 ? x / repetition[r] : x * repetition[r];
+ *   n = times w occurs in the generated part of the history and on the path: x -= frequency[r] * n + (n > 0 ? presence[r] : 0);
+ *   x += bias of w, if it has one (the last entry counts); x = -inf where bit w of the row's grammar mask is 0.
+ * The policy's arrays are per request: history ids packed by history_offsets [requests + 1] (absolute; the first
+ * prompt_lengths[r] of them are the prompt's), bias entries packed by bias_offsets; history, repetition, presence, frequency and
+ * the bias arrays may be NULL. The drafts are those of a step: row t belongs to row_request[t] (NULL: request t; a negative one is
+ * padding and its row of out is left as it was), drafted[t] is the word that was fed for row t (NULL: no paths), and the path of a row
+ * are the drafted words of its ancestors and itself. Negative words are padding. logits and out have `qtype` F32, F16 or BF16 with strides in elements; out may be
+ * logits. grammar: [rows] bit masks of grammar_stride words of 32 bits, NULL for none. Arithmetic is f32, rounded once. Status 1: a NaN in an allowed place; 2: a word or
+ * request out of range, offsets that decrease or pass the packed arrays' lengths, a repetition that is not positive and finite (it counts as 1).
+ */
+typedef struct yvex_b200_logits_policy {
+    uint64_t vocabulary, requests, history_tokens, bias_entries;    /* the last two: lengths of the packed arrays */
+    const int32_t *history, *history_offsets, *prompt_lengths;
+    const float *repetition, *presence, *frequency;
+    const int32_t *bias_tokens;
+    const float *bias_values;
+    const int32_t *bias_offsets;
+} yvex_b200_logits_policy;
+typedef struct yvex_b200_logits_drafts {
+    uint64_t rows;
+    int tree;
+    const int32_t *drafted, *row_request, *offsets;
+    const uint64_t *ancestors;
+} yvex_b200_logits_drafts;
+int yvex_b200_logits_edit(const yvex_b200_logits_policy *policy, const yvex_b200_logits_drafts *drafts, unsigned int qtype,
+                          const void *logits, uint64_t logits_stride, const uint32_t *grammar, uint64_t grammar_stride,
+                          void *out, uint64_t out_stride, int *status, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -46,6 +46,28 @@ class Mhc(C.Structure):
                 ("base", vp), ("norm", vp)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("qtype", u32), ("pages", u64), ("page_size", u64), ("kv_heads", u64), ("head_dim", u64), ("k", vp), ("v", vp)]
+
+
+class KvStep(C.Structure):
+    _fields_ = [("requests", u64), ("tokens", u64), ("table_width", u64), ("longest_fresh", u64), ("longest", u64), ("tree", C.c_int),
+                ("cached", vp), ("fresh", vp), ("parents", vp), ("block_table", vp), ("offsets", vp), ("slots", vp), ("positions", vp),
+                ("row_request", vp), ("ancestors", vp)]
+
+
+class LogitsPolicy(C.Structure):
+    _fields_ = [("vocabulary", u64), ("requests", u64), ("history_tokens", u64), ("bias_entries", u64), ("history", vp), ("history_offsets", vp), ("prompt_lengths", vp), ("repetition", vp),
+                ("presence", vp), ("frequency", vp), ("bias_tokens", vp), ("bias_values", vp), ("bias_offsets", vp)]
+
+
+class LogitsDrafts(C.Structure):
+    _fields_ = [("rows", u64), ("tree", C.c_int), ("drafted", vp), ("row_request", vp), ("offsets", vp), ("ancestors", vp)]
+
+
+TREE_NODES = 64                # YVEX_B200_TREE_NODES
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is missing: run `python -m yvex_b200.build` (there is no fallback path)")
@@ -104,6 +126,12 @@ def _load():
     lib.yvex_b200_attention_static_scratch_bytes.argtypes = []
     lib.yvex_b200_attention_gqa_decode_static.argtypes = [vp, vp, vp, u64, u64, u64, u64, u64, u64, C.c_float,
                                                           vp, vp, vp]
+    lib.yvex_b200_kv_plan.argtypes = [C.POINTER(KvCache), C.POINTER(KvStep), vp, u64, vp, vp, vp]
+    lib.yvex_b200_kv_append.argtypes = [C.POINTER(KvCache), vp, u64, C.c_uint, vp, u64, vp, u64, vp, vp]
+    lib.yvex_b200_attention_paged_workspace_bytes.restype = u64
+    lib.yvex_b200_attention_paged_workspace_bytes.argtypes = [C.POINTER(KvCache), C.POINTER(KvStep), u64]
+    lib.yvex_b200_attention_paged.argtypes = [C.POINTER(KvCache), C.POINTER(KvStep), vp, u64, u64, C.c_float, vp, vp, u64, vp, vp]
+    lib.yvex_b200_logits_edit.argtypes = [C.POINTER(LogitsPolicy), C.POINTER(LogitsDrafts), C.c_uint, vp, u64, vp, u64, vp, u64, vp, vp]
     return lib
 
 
@@ -124,7 +152,8 @@ EXPORTS = ["yvex_b200_version", "yvex_b200_qtype_supported", "yvex_b200_qtype_ge
            "yvex_b200_moe_wide_set_cta_limit", "yvex_b200_moe_decode_parts", "yvex_b200_moe_wide_parts",
            "yvex_b200_dequant_gather", "yvex_b200_q8k_round_trip", "yvex_b200_concat_bf16",
            "yvex_b200_moe_expert_rows_scatter", "yvex_b200_ep_dispatch_plan", "yvex_b200_ep_dispatch_push",
-           "yvex_b200_moe_expert_rows_sorted"]
+           "yvex_b200_moe_expert_rows_sorted", "yvex_b200_kv_plan", "yvex_b200_kv_append",
+           "yvex_b200_attention_paged_workspace_bytes", "yvex_b200_attention_paged", "yvex_b200_logits_edit"]
 
 
 _module = None
@@ -487,3 +516,162 @@ def attention_f32(q, keys, values, position, scale, causal, status):
     _check(lib.yvex_b200_attention_f32(_p(q), _p(keys), _p(values), seq, D, position, scale, int(causal),
                                        _p(scores), _p(probs), _p(out), _p(status.word), _stream()), "attention_f32")
     return out, scores, probs
+
+
+# ---- a serving step over a paged cache --------------------------------------------------------------------------------
+
+INVALID_ARG, UNSUPPORTED = -10, -5
+
+
+def _qtype_of(t, where):
+    """GGUF id of a tensor's type (F32, F16, BF16)."""
+    torch = _torch()
+    q = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}.get(t.dtype)
+    if q is None:
+        raise YvexError(UNSUPPORTED, where)
+    return q
+
+
+def _need(ok, where):
+    if not ok:
+        raise YvexError(INVALID_ARG, where)
+
+
+def _here(t):
+    """The tensor lies on the current device, whose current stream the call goes to."""
+    return t.is_cuda and t.get_device() == _torch().cuda.current_device()
+
+
+def _array(t, dtype, numel, where):
+    """A packed device array of the given type with at least `numel` elements (None: whatever it has), or None."""
+    _need(t is None or (t.dtype == dtype and t.is_contiguous() and _here(t) and (numel is None or t.numel() >= numel)), where)
+    return _p(t)
+
+
+def _row_stride(t, where):
+    """Elements between the rows of [rows, heads, dim] values whose rows are packed."""
+    rows, heads, dim = t.shape
+    _need((t.stride(2) == 1 or dim == 1) and (t.stride(1) == dim or heads == 1), where)
+    return t.stride(0) if rows > 1 else heads * dim
+
+
+def kv_geometry_of(pages, page_size):
+    """A cache as far as a plan reads it: the number of its pages and of the tokens in each."""
+    return KvCache(0, pages, page_size, 0, 0, None, None)
+
+
+def kv_cache_of(k, v):
+    """Description of a paged cache: k, v [pages, kv_heads, page_size, head_dim] of f16 or bf16, packed."""
+    _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous() and _here(k) and _here(v), "kv_cache_of")
+    pages, heads, page_size, dim = k.shape
+    c = KvCache(_qtype_of(k, "kv_cache_of"), pages, page_size, heads, dim, _p(k), _p(v))
+    c._keep, c.dtype = (k, v), k.dtype
+    return c
+
+
+def kv_step_of(cached, fresh, block_table, tokens, longest_fresh, longest, parents=None, tree=None, offsets=None, slots=None, positions=None,
+               row_request=None, ancestors=None):
+    """Description of a serving step over int32 device arrays: cached, fresh [requests], block_table [requests, width], parents
+    [tokens] for drafted trees. The arrays that kv_plan writes (offsets [requests + 1], slots int64, positions, row_request [tokens],
+    ancestors int64 [tokens] for trees) are made here unless given; they are the step's *_tensor attributes."""
+    torch = _torch()
+    tree = bool(tree if tree is not None else parents is not None)
+    requests, dev, i32, i64, w = cached.numel(), cached.device, torch.int32, torch.int64, "kv_step_of"
+    _need(block_table.dim() == 2 and block_table.shape[0] == requests, w)
+    new = lambda t, n, dtype: torch.empty(n, dtype=dtype, device=dev) if t is None else t  # noqa: E731
+    offsets, slots = new(offsets, requests + 1, i32), new(slots, tokens, i64)
+    positions, row_request = new(positions, tokens, i32), new(row_request, tokens, i32)
+    ancestors = new(ancestors, tokens, i64) if tree else None
+    s = KvStep(requests, tokens, block_table.shape[1], longest_fresh, longest, int(tree), _array(cached, i32, requests, w), _array(fresh, i32, requests, w),
+               _array(parents, i32, tokens, w), _array(block_table, i32, None, w), _array(offsets, i32, requests + 1, w), _array(slots, i64, tokens, w),
+               _array(positions, i32, tokens, w), _array(row_request, i32, tokens, w), _array(ancestors, i64, tokens, w))
+    s._keep = (cached, fresh, parents, block_table)
+    s.offsets_tensor, s.slots_tensor, s.positions_tensor, s.row_request_tensor, s.ancestors_tensor = offsets, slots, positions, row_request, ancestors
+    return s
+
+
+def kv_plan(cache, step, free_pages, status, pages_used=None):
+    """Plans the step on the device (see yvex_b200_kv_plan); free_pages int32 -> pages_used [1] int32, how many of them it took."""
+    torch = _torch()
+    if pages_used is None:
+        pages_used = torch.empty(1, dtype=torch.int32, device=free_pages.device)
+    _check(lib.yvex_b200_kv_plan(cache, step, _array(free_pages, torch.int32, None, "kv_plan"), free_pages.numel(),
+                                 _array(pages_used, torch.int32, 1, "kv_plan"), _p(status.word), _stream()), "kv_plan")
+    return pages_used
+
+
+def kv_append(cache, slots, k, v, status):
+    """Stores rows k, v [tokens, kv_heads, head_dim] (f32, f16 or bf16; rows may be strided views, as of a fused projection) at
+    slots [tokens] int64; negative slots are skipped."""
+    torch, w = _torch(), "kv_append"
+    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
+    _need(k.shape == shape and v.shape == shape and k.dtype == v.dtype and _here(k) and _here(v), w)
+    _check(lib.yvex_b200_kv_append(cache, _array(slots, torch.int64, None, w), slots.numel(), _qtype_of(k, w), _p(k), _row_stride(k, w), _p(v),
+                                   _row_stride(v, w), _p(status.word), _stream()), w)
+
+
+def attention_paged_workspace(cache, step, q_heads):
+    """Scratch for attention_paged calls of this cache and step sizes."""
+    torch = _torch()
+    n = int(lib.yvex_b200_attention_paged_workspace_bytes(cache, step, q_heads))
+    _need(n > 0, "attention_paged_workspace")
+    return torch.empty(n, dtype=torch.uint8, device="cuda")
+
+
+def attention_paged(cache, step, q, scale, status, workspace=None, out=None):
+    """q [tokens, q_heads, head_dim] in the cache's type (rows may be strided) -> out [tokens, q_heads, head_dim] in the same type."""
+    torch, w = _torch(), "attention_paged"
+    _need(q.dim() == 3 and q.shape[0] == step.tokens and q.shape[2] == cache.head_dim and q.dtype == cache.dtype and _here(q), w)
+    heads = q.shape[1]
+    if workspace is None:
+        workspace = attention_paged_workspace(cache, step, heads)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _check(lib.yvex_b200_attention_paged(cache, step, _p(q), _row_stride(q, w), heads, scale, _array(out, q.dtype, q.numel(), w),
+                                         _array(workspace, torch.uint8, None, w), workspace.numel(), _p(status.word), _stream()), w)
+    return out
+
+
+def logits_policy_of(vocabulary, history=None, history_offsets=None, prompt_lengths=None, repetition=None, presence=None, frequency=None,
+                     bias_tokens=None, bias_values=None, bias_offsets=None, requests=None):
+    """What the requests' logits are edited by: ids int32 packed by offsets [requests + 1] int32, penalties [requests] f32."""
+    torch, w = _torch(), "logits_policy_of"
+    i32, f32 = torch.int32, torch.float32
+    if requests is None:
+        known = [t.numel() - 1 for t in (history_offsets, bias_offsets) if t is not None] +                 [t.numel() for t in (prompt_lengths, repetition, presence, frequency) if t is not None]
+        _need(known, w)
+        requests = known[0]
+    count = lambda t: 0 if t is None else t.numel()  # noqa: E731
+    p = LogitsPolicy(vocabulary, requests, count(history), count(bias_tokens), _array(history, i32, None, w), _array(history_offsets, i32, requests + 1, w),
+                     _array(prompt_lengths, i32, requests, w), _array(repetition, f32, requests, w), _array(presence, f32, requests, w),
+                     _array(frequency, f32, requests, w), _array(bias_tokens, i32, None, w),
+                     _array(bias_values, f32, count(bias_tokens), w), _array(bias_offsets, i32, requests + 1, w))
+    p._keep = (history, history_offsets, prompt_lengths, repetition, presence, frequency, bias_tokens, bias_values, bias_offsets)
+    return p
+
+
+def logits_drafts_of(drafted=None, row_request=None, offsets=None, ancestors=None, tree=False, rows=None):
+    """Which request each row of logits belongs to, and the words drafted for the rows (arrays as kv_plan writes them)."""
+    torch, w = _torch(), "logits_drafts_of"
+    if rows is None:
+        _need(row_request is not None, w)
+        rows = row_request.numel()
+    d = LogitsDrafts(rows, int(tree), _array(drafted, torch.int32, rows, w), _array(row_request, torch.int32, rows, w),
+                     _array(offsets, torch.int32, None, w), _array(ancestors, torch.int64, rows, w))
+    d._keep, d.requests = (drafted, row_request, offsets, ancestors), None if offsets is None else offsets.numel() - 1
+    return d
+
+
+def logits_edit(policy, drafts, logits, status, grammar=None, out=None):
+    """logits [rows, vocabulary] f32, f16 or bf16 -> the edited rows (out may be logits itself); grammar [rows, words] int32 bit masks."""
+    torch, w = _torch(), "logits_edit"
+    _need(logits.dim() == 2 and logits.shape[0] >= drafts.rows and logits.shape[1] == policy.vocabulary and logits.stride(1) == 1 and _here(logits), w)
+    _need(drafts.requests is None or drafts.requests >= policy.requests, w)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _need(out.shape == logits.shape and out.dtype == logits.dtype and out.stride(1) == 1 and _here(out), w)
+    if grammar is not None:
+        _need(grammar.dim() == 2 and grammar.shape[0] >= drafts.rows and grammar.dtype == torch.int32 and grammar.stride(1) == 1 and _here(grammar), w)
+    _check(lib.yvex_b200_logits_edit(policy, drafts, _qtype_of(logits, w), _p(logits), logits.stride(0), _p(grammar),
+                                     grammar.stride(0) if grammar is not None else 0, _p(out), out.stride(0), _p(status.word), _stream()), w)
+    return out
