@@ -1,98 +1,339 @@
 // Attention of a step's fresh tokens over the paged cache: softmax(scale q K^T) V with one running maximum and sum per row.
-#include "paged.cuh"
+//
+// Few rows per (request, kv head) - one token of a group of query heads, a short chain -: bound by HBM, the cache is read once and
+// the products hide behind it. Like the contiguous decode kernel, a warp takes 16 keys at a time and does both products on
+// mma.sync m16n8k16 with operands built from 16-byte loads as they lie in memory (the k-slots of S are whatever dims, those
+// of PV whatever keys a lane holds), so nothing is staged or transposed. 16 keys never straddle a page, and the page
+// of a warp's next block is looked up while this one is computed. The weights are rounded once to the cache's type for the second product,
+// which adds less to the output's error than its own rounding (an output of f32 would not allow that); their sum stays f32 and unrounded.
+#include <cuda_bf16.h>
+
+#include <initializer_list>
+
+#include "paged_work.cuh"
 
 namespace yb {
 
-struct PagedParams {
-    const uint16_t *q, *k, *v;
-    uint16_t *out;
-    uint64_t q_stride, pages, page_size, table_width, requests, tokens, longest_fresh, longest;
-    uint32_t kv_heads, group;
-    int tree;
-    const int32_t *cached, *offsets, *block_table;
-    const uint64_t *ancestors;
-    float scale;
-    int *status;
-};
+int launch_paged_tiles(const PagedParams &p, unsigned qtype, uint64_t head_dim, unsigned ctas, cudaStream_t s);
 
-template <class T> __device__ __forceinline__ float2 open2(uint32_t w) {
-    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+constexpr int kRowsThreads = 128, kRowsWarps = kRowsThreads / 32;
+constexpr int kRowsBlock = 16 * kRowsWarps;                     // keys of a unit of work: 16 a warp
+
+template <class T> __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <class T> __device__ __forceinline__ uint32_t close2(float a, float b) {
-    if constexpr (std::is_same<T, __half>::value) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
-    else { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+__device__ __forceinline__ uint4 ldg_once(const uint16_t *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
 }
 
-// One warp per (row, query head), one key after the other.
-template <class T, int D>
-__global__ void __launch_bounds__(256) paged_rows_kernel(const PagedParams p) {
-    constexpr int W = D / 64;                           // 32-bit words of a row per lane
+// R: rows held, 8 or 16 (the MMA has 16; with 8 the upper ones are zero and their results dropped).
+template <class T, int D, int R>
+__global__ void __launch_bounds__(kRowsThreads, R == 8 && D <= 128 ? 3 : 2) paged_rows_kernel(const PagedParams p) {
+    constexpr int KL = D / 32, VU = D / 64, H = R / 8;
+    __shared__ uint64_t s_scan[kRowsWarps + 4];
+    __shared__ float s_m[kRowsWarps][R], s_l[kRowsWarps][R];
+    __shared__ float s_acc[kRowsWarps][R][D];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     pdl_trigger();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31u, q_heads = p.kv_heads * p.group;
-    const uint64_t job = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    const uint64_t row = job / q_heads;
-    const uint32_t head = (uint32_t)(job % q_heads), kvh = head / p.group;
-    if (row >= p.tokens) return;
-    uint64_t lo = 0, hi = p.requests - 1;
-    if ((int64_t)row >= p.offsets[p.requests]) return;
-    while (lo < hi) {
-        const uint64_t mid = (lo + hi + 1) / 2;
-        if (p.offsets[mid] <= (int64_t)row) lo = mid; else hi = mid - 1;
-    }
-    const int64_t begin = p.offsets[lo], fresh = p.offsets[lo + 1] - begin, cached = max(p.cached[lo], 0), index = (int64_t)row - begin;
-    bool bad = p.cached[lo] < 0 || begin < 0 || index < 0 || fresh > (int64_t)p.longest_fresh || cached + fresh > (int64_t)p.longest || index >= fresh;
-    const int64_t room = (int64_t)(p.table_width * p.page_size);
-    bad |= cached + fresh > room;
-    if (bad) { if (lane == 0) raise(p.status, YVEX_B200_STATUS_ARGUMENT); return; }
-    const uint64_t mask = p.tree ? p.ancestors[row] : 0ull;
-    const int64_t visible = p.tree ? cached + fresh : cached + index + 1;
-    float2 q[W], acc[W];
-    const uint32_t *qr = reinterpret_cast<const uint32_t *>(p.q + row * p.q_stride + (uint64_t)head * D);
+    const PagedStart start = paged_start<kRowsThreads, R, kRowsBlock>(p, s_scan);
+    PagedWalk<R, kRowsBlock> w;
+    const uint32_t units_per_page = (uint32_t)(p.page_size / 16);
+    const float scale = p.scale * 1.4426950408889634f;          // scores in powers of two
+    if (tid == 0) p.share[blockIdx.x].rows = 0;
+    bool bad_page = false, bad_out = false;
+
+    for (w.start(p, start); w.live(); w.next(p)) {
+        const int64_t cached = w.q.n.cached, end = (int64_t)w.q.n.cached + w.q.n.fresh;
+        const int32_t *table = p.block_table + (uint64_t)w.request * p.table_width;
+        const uint64_t head_at = (uint64_t)w.head * p.page_size, pitch = (uint64_t)p.kv_heads * p.page_size;
+        // ---- the rows: lane (g, c) holds dims 8 (c + 4 i) .. of rows g and g + 8
+        uint32_t qa[H][KL][4];
+        int64_t seen[H];
+        uint64_t mask[H];
 #pragma unroll
-    for (int i = 0; i < W; ++i) { q[i] = open2<T>(qr[lane + 32 * i]); acc[i] = make_float2(0.0f, 0.0f); }
-    float m = -INFINITY, l = 0.0f;
-    for (int64_t j = 0; j < visible; ++j) {
-        if (p.tree && j >= cached && (j - cached > 63 || !((mask >> (j - cached)) & 1ull))) continue;
-        const int32_t page = p.block_table[lo * p.table_width + (uint64_t)j / p.page_size];
-        if (page < 0 || (uint64_t)page >= p.pages) { bad = true; continue; }
-        const uint64_t at = (((uint64_t)page * p.kv_heads + kvh) * p.page_size + (uint64_t)j % p.page_size) * D;
-        const uint32_t *kr = reinterpret_cast<const uint32_t *>(p.k + at), *vr = reinterpret_cast<const uint32_t *>(p.v + at);
-        float s = 0.0f;
+        for (int h = 0; h < H; ++h) {
+            const uint32_t row = (uint32_t)(g + 8 * h), token = row / p.group;
+            const bool live = row < w.q.rows;
+            const uint16_t *src = p.q + (uint64_t)(w.q.n.token + token) * p.q_stride + ((uint64_t)w.head * p.group + row % p.group) * D;
 #pragma unroll
-        for (int i = 0; i < W; ++i) { const float2 x = open2<T>(kr[lane + 32 * i]); s += q[i].x * x.x + q[i].y * x.y; }
-        s = warp_sum(s) * p.scale;
-        const float top = fmaxf(m, s);
-        if (s != s || top == INFINITY) { l = NAN; continue; }
-        if (top == -INFINITY) continue;
-        const float c = expf(m - top), w = expf(s - top);
-        m = top;
-        l = l * c + w;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            const float2 x = open2<T>(vr[lane + 32 * i]);
-            acc[i].x = acc[i].x * c + w * x.x;
-            acc[i].y = acc[i].y * c + w * x.y;
+            for (int i = 0; i < KL; ++i) {
+                const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src) + c + 4 * i) : make_uint4(0, 0, 0, 0);
+                qa[h][i][0] = v.x; qa[h][i][1] = v.y; qa[h][i][2] = v.z; qa[h][i][3] = v.w;
+            }
+            seen[h] = live ? cached + token + 1 : cached;
+            mask[h] = p.tree && live ? p.ancestors[w.q.n.token + token] : 0ull;
         }
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    bool odd = false;
-    uint32_t *o = reinterpret_cast<uint32_t *>(p.out + (row * q_heads + head) * D);
+        float m[H], l[H], acc[VU][8][4];
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-        const float x = acc[i].x * inv, y = acc[i].y * inv;
-        odd |= !isfinite(x) || !isfinite(y);
-        o[lane + 32 * i] = close2<T>(x, y);
+        for (int h = 0; h < H; ++h) { m[h] = -INFINITY; l[h] = 0.0f; }
+#pragma unroll
+        for (int u = 0; u < VU; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[u][j][e] = 0.0f;
+
+        auto page_of = [&](int64_t base) -> int32_t {           // the page of the 16 keys from base on; -1 past the end
+            return base < end ? __ldg(table + (uint32_t)(base / 16) / units_per_page) : -1;
+        };
+        int64_t base = (int64_t)w.first * kRowsBlock + 16 * warp;
+        int32_t page = page_of(base);
+        for (uint32_t i = 0; i < w.count; ++i, base += kRowsBlock) {
+            const int32_t ahead = i + 1 < w.count ? page_of(base + kRowsBlock) : -1;
+            const bool fine = page >= 0 && (uint64_t)page < p.pages;
+            if (base < end && !fine) bad_page = true;
+            const int64_t stop = fine ? end : base;             // keys from here on are not read
+            const uint64_t at = ((uint64_t)(fine ? page : 0) * pitch + head_at + ((uint32_t)(base / 16) % units_per_page) * 16u) * D;
+            const uint16_t *kb = p.k + at, *vb = p.v + at;
+            page = ahead;
+            if (base >= stop) continue;
+            uint4 kr[2][KL], vr[4][VU];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int key = 8 * half + g;
+#pragma unroll
+                for (int x = 0; x < KL; ++x) kr[half][x] = base + key < stop ? ldg_once(kb + key * D + 8 * (c + 4 * x)) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int key = 2 * c + (r & 1) + 8 * (r >> 1);
+#pragma unroll
+                for (int u = 0; u < VU; ++u) vr[r][u] = base + key < stop ? ldg_once(vb + key * D + 8 * (g + 8 * u)) : make_uint4(0, 0, 0, 0);
+            }
+            // ---- S: sc[half] = scores of rows g (0, 1) and g + 8 (2, 3), keys base + 8 half + 2c, + 1
+            float sc[2][4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[half][e] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < KL; ++x) {
+                    const uint32_t b[4] = {kr[half][x].x, kr[half][x].y, kr[half][x].z, kr[half][x].w};
+                    mma16816<T>(sc[half], qa[0][x][0], H == 2 ? qa[H - 1][x][0] : 0u, qa[0][x][1], H == 2 ? qa[H - 1][x][1] : 0u, b[0], b[1]);
+                    mma16816<T>(sc[half], qa[0][x][2], H == 2 ? qa[H - 1][x][2] : 0u, qa[0][x][3], H == 2 ? qa[H - 1][x][3] : 0u, b[2], b[3]);
+                }
+            }
+            // ---- keys that not every row sees: fresh ones, and the block's end
+            uint32_t sees[H], odd = 0;
+#pragma unroll
+            for (int h = 0; h < H; ++h) sees[h] = 0xffffu;
+            if (base + 16 > cached) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) sees[h] = (uint32_t)(paged_sees(p.tree, base, cached, seen[h], mask[h]) & low_bits(end - base)) & 0xffffu;
+                // a weight of zero times an infinity would reach rows that do not see it: such values are taken out, and rows that see them marked
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int key = 2 * c + (r & 1) + 8 * (r >> 1);
+                    if (base + key < cached) continue;
+#pragma unroll
+                    for (int u = 0; u < VU; ++u) {
+                        uint32_t *x = reinterpret_cast<uint32_t *>(&vr[r][u]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t o = odd_halves<T>(x[e]);
+                            if (o) { odd |= 1u << key; x[e] = without_halves(x[e], o); }
+                        }
+                    }
+                }
+                odd = __reduce_or_sync(0xffffffffu, odd);
+            }
+            // ---- softmax of the block, P as A fragments
+            uint32_t pa[2][2] = {{0u, 0u}, {0u, 0u}};           // [half][rows g, rows g + 8]
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                float x[2][2], top = m[h];
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        x[half][e] = (sees[h] >> (8 * half + 2 * c + e)) & 1u ? sc[half][2 * h + e] * scale : -INFINITY;
+                        top = fmaxf(top, x[half][e]);
+                    }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float shift = top == -INFINITY ? 0.0f : top, corr = exp2f(m[h] - shift);
+                m[h] = top;
+                l[h] *= corr;
+                if (corr != 1.0f) {
+#pragma unroll
+                    for (int u = 0; u < VU; ++u)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) { acc[u][j][2 * h] *= corr; acc[u][j][2 * h + 1] *= corr; }
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float p0 = exp2f(x[half][0] - shift), p1 = exp2f(x[half][1] - shift);
+                    pa[half][h] = close2<T>(p0, p1);
+                    l[h] += p0 + p1;
+                }
+                if (odd & sees[h]) l[h] = NAN;
+            }
+            // ---- O += P V: n-tile (u, j) is dim j of chunks 8u .. 8u + 7, the k-slots are this lane's keys
+#pragma unroll
+            for (int u = 0; u < VU; ++u) {
+                const uint32_t r0[4] = {vr[0][u].x, vr[0][u].y, vr[0][u].z, vr[0][u].w}, r1[4] = {vr[1][u].x, vr[1][u].y, vr[1][u].z, vr[1][u].w};
+                const uint32_t r2[4] = {vr[2][u].x, vr[2][u].y, vr[2][u].z, vr[2][u].w}, r3[4] = {vr[3][u].x, vr[3][u].y, vr[3][u].z, vr[3][u].w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+                    mma16816<T>(acc[u][j], pa[0][0], pa[0][1], pa[1][0], pa[1][1], __byte_perm(r0[j >> 1], r1[j >> 1], sel),
+                                __byte_perm(r2[j >> 1], r3[j >> 1], sel));
+                }
+            }
+        }
+        // ---- the warps' states joined
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            if (c == 0) { s_m[warp][g + 8 * h] = m[h]; s_l[warp][g + 8 * h] = l[h]; }
+#pragma unroll
+            for (int u = 0; u < VU; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) s_acc[warp][g + 8 * h][8 * (2 * c + e + 8 * u) + j] = acc[u][j][2 * h + e];
+        }
+        __syncthreads();
+        const bool whole = w.begins && w.ends;
+        float *slot = p.partial + (2ull * blockIdx.x + (w.begins ? 1 : 0)) * R * (D + 2);
+        for (int idx = tid; idx < (int)w.q.rows * (D / 2); idx += kRowsThreads) {
+            const int row = idx / (D / 2), d = 2 * (idx % (D / 2));
+            float top = -INFINITY, sum = 0.0f, a = 0.0f, b = 0.0f;
+#pragma unroll
+            for (int x = 0; x < kRowsWarps; ++x) top = fmaxf(top, s_m[x][row]);
+#pragma unroll
+            for (int x = 0; x < kRowsWarps; ++x) {
+                const float f = s_m[x][row] == -INFINITY ? 0.0f : exp2f(s_m[x][row] - top);
+                sum += s_m[x][row] == -INFINITY ? s_l[x][row] : s_l[x][row] * f;     // (a NaN sum marks the row whatever its maximum)
+                a += s_acc[x][row][d] * f;
+                b += s_acc[x][row][d + 1] * f;
+            }
+            if (whole) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                a *= inv;
+                b *= inv;
+                bad_out |= !isfinite(a) || !isfinite(b);
+                const uint64_t token = w.q.n.token + (uint32_t)row / p.group, head = (uint64_t)w.head * p.group + (uint32_t)row % p.group;
+                *reinterpret_cast<uint32_t *>(p.out + (token * p.kv_heads * p.group + head) * D + d) = close2<T>(a, b);
+            } else {
+                if (d == 0) { slot[2 * row] = top; slot[2 * row + 1] = sum; }
+                *reinterpret_cast<float2 *>(slot + 2 * R + row * D + d) = make_float2(a, b);
+            }
+        }
+        if (tid == 0 && w.begins && !w.ends)
+            p.share[blockIdx.x] = PagedShare{w.last_cta(start), (int32_t)w.q.rows, (int32_t)w.q.n.token, (int32_t)(w.head * p.group), 0, {0, 0, 0}};
+        __syncthreads();
     }
-    if (bad) raise(p.status, YVEX_B200_STATUS_ARGUMENT);
-    if (odd) raise(p.status, YVEX_B200_STATUS_NUMERIC);
+    if (bad_page) raise(p.status, YVEX_B200_STATUS_ARGUMENT);
+    if (bad_out) raise(p.status, YVEX_B200_STATUS_NUMERIC);
 }
 
-template <class T, int D> static int launch_rows(const PagedParams &p, cudaStream_t s) {
-    const uint64_t warps = p.tokens * p.kv_heads * p.group;
-    if (launch_pdl(paged_rows_kernel<T, D>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, p) != cudaSuccess) return ERR_BACKEND;
-    return launch_status(1);
+// Joins the parts of the item that CTA blockIdx.x of the kernel before began and did not end: a warp per row. The parts' (maximum, sum)
+// pairs are read by one lane each, so their factors are known after one load each and the partial rows are independent loads.
+constexpr int kJoinWarps = 4;
+template <class T, int D>
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const PagedParams p, int slot_rows) {
+    constexpr int N = D / 32;
+    pdl_trigger();
+    pdl_wait();
+    const PagedShare sh = p.share[blockIdx.x];
+    const int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= sh.rows) return;
+    const uint64_t pitch = (uint64_t)slot_rows * (D + 2);
+    const int parts = sh.last - (int)blockIdx.x + 1;
+    auto slot = [&](int i) { return p.partial + (2ull * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * pitch; };
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, slot(i)[2 * row]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.0f, acc[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] = 0.0f;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        float m = -INFINITY, l = 0.0f;
+        if (i0 + lane < parts) {
+            const float2 v = *reinterpret_cast<const float2 *>(slot(i0 + lane) + 2 * row);
+            m = v.x; l = v.y;
+        }
+        const float mine = m == -INFINITY ? 0.0f : exp2f(m - top);
+        sum += m == -INFINITY ? l : l * mine;
+        const int n = min(32, parts - i0);
+        for (int i = 0; i < n; i += 4) {
+            float x[4][N];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float *src = slot(i0 + min(i + k, n - 1)) + 2 * slot_rows + (uint64_t)row * D;
+#pragma unroll
+                for (int j = 0; j < N; ++j) x[k][j] = src[lane + 32 * j];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float f = i + k < n ? __shfl_sync(0xffffffffu, mine, (i + k) & 31) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; ++j) acc[j] += i + k < n ? x[k][j] * f : 0.0f;
+            }
+        }
+    }
+    sum = warp_sum(sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const uint32_t r = (uint32_t)(sh.first_row + row);
+    const uint64_t token = (uint64_t)sh.token + r / p.group, head = (uint64_t)sh.head + r % p.group;
+    T *o = reinterpret_cast<T *>(p.out) + (token * p.kv_heads * p.group + head) * D;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float y = acc[j] * inv;
+        bad |= !isfinite(y);
+        if constexpr (std::is_same<T, __half>::value) o[lane + 32 * j] = __float2half_rn(y);
+        else o[lane + 32 * j] = __float2bfloat16_rn(y);
+    }
+    if (bad) raise(p.status, YVEX_B200_STATUS_NUMERIC);
+}
+
+// Which kernel, for how many rows a slot holds, on how many CTAs. Up to 16 rows fit the MMA of the rows kernel (8 with 256 dims, where
+// sixteen rows of Q and O would not fit the registers).
+struct PagedShape { bool tiles; uint32_t rows; unsigned ctas; };
+static PagedShape paged_shape(const yvex_b200_kv_cache *c, const yvex_b200_kv_step *t, uint64_t q_heads) {
+    const uint64_t group = q_heads / c->kv_heads, rows = t->longest_fresh * group, D = c->head_dim;
+    PagedShape s;
+    s.tiles = rows > (D == 256 ? 8u : 16u);
+    s.rows = s.tiles ? (D == 256 ? 128u : 256u) : rows <= 8 ? 8u : 16u;
+    const uint64_t keys = s.tiles ? (D == 256 ? 64u : 128u) : (uint64_t)kRowsBlock;
+    // no more CTAs than there can be blocks of keys
+    const uint64_t tiles = (rows + s.rows - 1) / s.rows, blocks = (t->longest + keys - 1) / keys;
+    uint64_t most = (uint64_t)kSmCount * (s.tiles ? 1u : s.rows == 8 && D <= 128 ? 3u : 2u);
+    for (uint64_t x : {t->requests, c->kv_heads, tiles, blocks}) if (x >= most) return s.ctas = (unsigned)most, s;
+    const uint64_t bound = t->requests * c->kv_heads * tiles * blocks;
+    s.ctas = (unsigned)(bound < most ? bound : most);
+    return s;
+}
+static uint64_t paged_partial_bytes(const PagedShape &s, uint64_t head_dim) {
+    return (2ull * s.ctas * s.rows * (head_dim + 2) * sizeof(float) + 255) / 256 * 256;
+}
+
+template <class T, int D> static int launch_paged(const PagedParams &p, const PagedShape &s, unsigned qtype, cudaStream_t stream) {
+    int rc = OK;
+    if (s.tiles) {
+        rc = launch_paged_tiles(p, qtype, D, s.ctas, stream);
+    } else if constexpr (D <= 128) {
+        if (launch_pdl(s.rows == 8 ? paged_rows_kernel<T, D, 8> : paged_rows_kernel<T, D, 16>, dim3(s.ctas), dim3(kRowsThreads), 0, stream, p) != cudaSuccess)
+            rc = ERR_BACKEND;
+    } else if (launch_pdl(paged_rows_kernel<T, D, 8>, dim3(s.ctas), dim3(kRowsThreads), 0, stream, p) != cudaSuccess) {
+        rc = ERR_BACKEND;
+    }
+    if (rc != OK) return rc;
+    if (launch_pdl(paged_join_kernel<T, D>, dim3(s.ctas, (s.rows + kJoinWarps - 1) / kJoinWarps), dim3(32 * kJoinWarps), 0, stream, p, (int)s.rows) != cudaSuccess)
+        return ERR_BACKEND;
+    return launch_status(2);
 }
 
 }  // namespace yb
@@ -104,12 +345,14 @@ static int paged_refusal(const yvex_b200_kv_cache *c, const yvex_b200_kv_step *t
     if (rc == OK) rc = check_step(t);
     if (rc != OK) return rc;
     if (!q_heads || q_heads % c->kv_heads) return ERR_INVALID_ARG;
-    if (q_heads > 65536) return ERR_BOUNDS;
+    if (q_heads > 65536 || c->pages * c->kv_heads * c->page_size > INT32_MAX) return ERR_BOUNDS;
     return OK;
 }
 
 extern "C" uint64_t yvex_b200_attention_paged_workspace_bytes(const yvex_b200_kv_cache *c, const yvex_b200_kv_step *t, uint64_t q_heads) {
-    return paged_refusal(c, t, q_heads) == OK ? 256 : 0;
+    if (paged_refusal(c, t, q_heads) != OK) return 0;
+    const PagedShape s = paged_shape(c, t, q_heads);
+    return paged_partial_bytes(s, c->head_dim) + s.ctas * sizeof(PagedShare);
 }
 
 extern "C" int yvex_b200_attention_paged(const yvex_b200_kv_cache *c, const yvex_b200_kv_step *t, const void *q, uint64_t q_stride, uint64_t q_heads,
@@ -120,13 +363,17 @@ extern "C" int yvex_b200_attention_paged(const yvex_b200_kv_cache *c, const yvex
     if (!isfinite(scale) || scale <= 0.0f) return ERR_INVALID_ARG;
     if (q_stride < q_heads * c->head_dim) return ERR_BOUNDS;
     if (((uintptr_t)q | (uintptr_t)out) & 15u || q_stride % 8) return ERR_INVALID_ARG;
-    if (!workspace || workspace_bytes < yvex_b200_attention_paged_workspace_bytes(c, t, q_heads)) return ERR_NOMEM;
+    const PagedShape s = paged_shape(c, t, q_heads);
+    const uint64_t partial = paged_partial_bytes(s, c->head_dim);
+    if (!workspace || workspace_bytes < partial + s.ctas * sizeof(PagedShare)) return ERR_NOMEM;
     if ((uintptr_t)workspace & 15u) return ERR_INVALID_ARG;
-    PagedParams p{(const uint16_t *)q, (const uint16_t *)c->k, (const uint16_t *)c->v, (uint16_t *)out, q_stride, c->pages, c->page_size, t->table_width,
-                  t->requests, t->tokens, t->longest_fresh, t->longest, (uint32_t)c->kv_heads, (uint32_t)(q_heads / c->kv_heads), t->tree != 0, t->cached,
-                  t->offsets, t->block_table, t->ancestors, scale, status};
-    cudaStream_t s = as_stream(stream);
-#define YB_ROWS(T) (c->head_dim == 64 ? launch_rows<T, 64>(p, s) : c->head_dim == 128 ? launch_rows<T, 128>(p, s) : launch_rows<T, 256>(p, s))
-    return c->qtype == Q_BF16 ? YB_ROWS(__nv_bfloat16) : YB_ROWS(__half);
-#undef YB_ROWS
+    const PagedParams p{(const uint16_t *)q, (const uint16_t *)c->k, (const uint16_t *)c->v, (uint16_t *)out, q_stride, c->pages, c->page_size,
+                        t->table_width, t->requests, t->tokens, t->longest_fresh, t->longest, (uint32_t)c->kv_heads, (uint32_t)(q_heads / c->kv_heads),
+                        t->tree != 0, t->cached, t->offsets, t->block_table, t->ancestors, scale, status, (float *)workspace,
+                        (PagedShare *)((char *)workspace + partial)};
+    cudaStream_t st = as_stream(stream);
+#define YB_PAGED(T) (c->head_dim == 64 ? launch_paged<T, 64>(p, s, c->qtype, st) : c->head_dim == 128 ? launch_paged<T, 128>(p, s, c->qtype, st) \
+                                       : launch_paged<T, 256>(p, s, c->qtype, st))
+    return c->qtype == Q_BF16 ? YB_PAGED(__nv_bfloat16) : YB_PAGED(__half);
+#undef YB_PAGED
 }

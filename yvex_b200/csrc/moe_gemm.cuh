@@ -303,13 +303,6 @@ template <class Dec> struct GemmPlan {
                   "TMA destinations are 128-byte aligned (boxes of 64 rows, up to 8 rows fused)");
 };
 
-// Sets this warpgroup's registers per thread to N, given the count the kernel was launched with. An
-// increase waits until other warpgroups of the CTA have handed enough registers back.
-template <int N, int kLaunched> __device__ __forceinline__ void set_registers() {
-    if constexpr (N > kLaunched) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-    else if constexpr (N < kLaunched) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 // a0 = d * v0 + a0, a1 = d * v1 + a1 in one instruction (each rounded like fmaf)
 __device__ __forceinline__ void fma2(float &a0, float &a1, float d, uint32_t v0, uint32_t v1) {
     asm("{\n\t.reg .b64 a, v, s;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\t"
