@@ -269,6 +269,26 @@ def test_attention_tree(L, which, shape, heads, group, dim, page, dtype):
     check_attention(s, out, q, k, v)
 
 
+@pytest.mark.parametrize("dtype,dim,group", [("bfloat16", 128, 4), ("float16", 64, 5), ("bfloat16", 256, 3), ("float16", 128, 7), ("bfloat16", 64, 2)])
+@pytest.mark.parametrize("tree", [None, "random"])
+@pytest.mark.parametrize("most", [1, 3, 64])
+def test_attention_many_requests(L, most, tree, dtype, dim, group):
+    """Shares of one CTA that hold ends, whole items and beginnings, of one tile of rows and of two, of requests with and without
+    fresh tokens; twice, with the same bits."""
+    import torch
+    rng = np.random.default_rng(most)
+    requests = 45
+    fresh = (rng.integers(1, most + 1, requests) * (rng.random(requests) < 0.9)).tolist()
+    fresh[0] = most
+    cached = (2500 * rng.random(requests) ** 3).astype(int).tolist()
+    s = Step(L, cached, fresh, 32, seed=most, tree=tree)
+    out, q, k, v, cache = attend(L, s, 4, group, dim, dtype, most)
+    assert s.status.read() == 0
+    check_attention(s, out, q, k, v)
+    again = L.attention_paged(cache, s.step, q, dim ** -0.5, s.status)
+    assert torch.equal(again[:sum(fresh)], out[:sum(fresh)])
+
+
 @pytest.mark.parametrize("scale", [1e-3, 3.0])
 @pytest.mark.parametrize("fresh", [1, 40])
 def test_attention_scales(L, scale, fresh):

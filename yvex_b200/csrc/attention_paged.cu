@@ -17,7 +17,7 @@ namespace yb {
 int launch_paged_tiles(const PagedParams &p, unsigned qtype, uint64_t head_dim, unsigned ctas, cudaStream_t s);
 
 constexpr int kRowsThreads = 128, kRowsWarps = kRowsThreads / 32;
-constexpr int kRowsBlock = 16 * kRowsWarps;                     // keys of a unit of work: 16 a warp
+constexpr int kRowsBlock = 16 * kRowsWarps, kRowsCost = 1;      // keys of a unit of work, 16 a warp; units that an item costs besides
 
 template <class T> __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same<T, __half>::value)
@@ -37,14 +37,14 @@ __device__ __forceinline__ uint4 ldg_once(const uint16_t *p) {
 template <class T, int D, int R>
 __global__ void __launch_bounds__(kRowsThreads, R == 8 && D <= 128 ? 3 : 2) paged_rows_kernel(const PagedParams p) {
     constexpr int KL = D / 32, VU = D / 64, H = R / 8;
-    __shared__ uint64_t s_scan[kRowsWarps + 4];
+    __shared__ PagedScratch<kRowsThreads> s_scan;
     __shared__ float s_m[kRowsWarps][R], s_l[kRowsWarps][R];
-    __shared__ float s_acc[kRowsWarps][R][D];
+    __shared__ __align__(16) float s_acc[kRowsWarps][R][D + 4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     pdl_trigger();
     pdl_wait();
-    const PagedStart start = paged_start<kRowsThreads, R, kRowsBlock>(p, s_scan);
-    PagedWalk<R, kRowsBlock> w;
+    const PagedStart start = paged_start<kRowsThreads, R, kRowsBlock, kRowsCost>(p, &s_scan);
+    PagedWalk<R, kRowsBlock, kRowsCost> w;
     const uint32_t units_per_page = (uint32_t)(p.page_size / 16);
     const float scale = p.scale * 1.4426950408889634f;          // scores in powers of two
     if (tid == 0) p.share[blockIdx.x].rows = 0;
@@ -204,29 +204,30 @@ __global__ void __launch_bounds__(kRowsThreads, R == 8 && D <= 128 ? 3 : 2) page
         }
         __syncthreads();
         const bool whole = w.begins && w.ends;
-        float *slot = p.partial + (2ull * blockIdx.x + (w.begins ? 1 : 0)) * R * (D + 2);
-        for (int idx = tid; idx < (int)w.q.rows * (D / 2); idx += kRowsThreads) {
-            const int row = idx / (D / 2), d = 2 * (idx % (D / 2));
-            float top = -INFINITY, sum = 0.0f, a = 0.0f, b = 0.0f;
+        float *slot = paged_slot(p, blockIdx.x, w.begins, R, D);
+        for (int idx = tid; idx < R * (D / 4); idx += kRowsThreads) {
+            const int row = whole ? idx / (D / 4) : idx % R, d = 4 * (whole ? idx % (D / 4) : idx / R);
+            if (row >= (int)w.q.rows) continue;
+            float top = -INFINITY, sum = 0.0f;
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int x = 0; x < kRowsWarps; ++x) top = fmaxf(top, s_m[x][row]);
 #pragma unroll
             for (int x = 0; x < kRowsWarps; ++x) {
                 const float f = s_m[x][row] == -INFINITY ? 0.0f : exp2f(s_m[x][row] - top);
                 sum += s_m[x][row] == -INFINITY ? s_l[x][row] : s_l[x][row] * f;     // (a NaN sum marks the row whatever its maximum)
-                a += s_acc[x][row][d] * f;
-                b += s_acc[x][row][d + 1] * f;
+                const float4 y = *reinterpret_cast<const float4 *>(&s_acc[x][row][d]);
+                a.x += y.x * f; a.y += y.y * f; a.z += y.z * f; a.w += y.w * f;
             }
             if (whole) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                a *= inv;
-                b *= inv;
-                bad_out |= !isfinite(a) || !isfinite(b);
+                a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
+                bad_out |= !isfinite(a.x) || !isfinite(a.y) || !isfinite(a.z) || !isfinite(a.w);
                 const uint64_t token = w.q.n.token + (uint32_t)row / p.group, head = (uint64_t)w.head * p.group + (uint32_t)row % p.group;
-                *reinterpret_cast<uint32_t *>(p.out + (token * p.kv_heads * p.group + head) * D + d) = close2<T>(a, b);
+                *reinterpret_cast<uint2 *>(p.out + (token * p.kv_heads * p.group + head) * D + d) = make_uint2(close2<T>(a.x, a.y), close2<T>(a.z, a.w));
             } else {
-                if (d == 0) { slot[2 * row] = top; slot[2 * row + 1] = sum; }
-                *reinterpret_cast<float2 *>(slot + 2 * R + row * D + d) = make_float2(a, b);
+                if (d == 0) *reinterpret_cast<float2 *>(slot + 2 * row) = make_float2(top, sum);
+                *reinterpret_cast<float4 *>(slot + 2 * R + (d / 4 * R + row) * 4) = a;
             }
         }
         if (tid == 0 && w.begins && !w.ends)
@@ -237,66 +238,39 @@ __global__ void __launch_bounds__(kRowsThreads, R == 8 && D <= 128 ? 3 : 2) page
     if (bad_out) raise(p.status, YVEX_B200_STATUS_NUMERIC);
 }
 
-// Joins the parts of the item that CTA blockIdx.x of the kernel before began and did not end: a warp per row. The parts' (maximum, sum)
-// pairs are read by one lane each, so their factors are known after one load each and the partial rows are independent loads.
-constexpr int kJoinWarps = 4;
+// Joins the parts of the item that CTA blockIdx.x of the kernel before began and did not end: a CTA takes eight rows, a thread four
+// columns of one of them (a warp's 8 rows x 16 columns are whole lines of every part, and whole sectors of the output). The parts are
+// walked twice, for their maximum and then for their sums; all loads of a walk are independent.
+constexpr int kJoinRows = 8;
 template <class T, int D>
-__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const PagedParams p, int slot_rows) {
-    constexpr int N = D / 32;
+__global__ void __launch_bounds__(2 * D) paged_join_kernel(const PagedParams p, int slot_rows) {
     pdl_trigger();
     pdl_wait();
     const PagedShare sh = p.share[blockIdx.x];
-    const int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, row = (int)blockIdx.y * kJoinRows + (lane >> 2), group = 4 * (threadIdx.x >> 5) + (lane & 3);
     if (row >= sh.rows) return;
-    const uint64_t pitch = (uint64_t)slot_rows * (D + 2);
+    const uint64_t pitch = paged_slot_floats((uint32_t)slot_rows, D);
     const int parts = sh.last - (int)blockIdx.x + 1;
     auto slot = [&](int i) { return p.partial + (2ull * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * pitch; };
     float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, slot(i)[2 * row]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.0f, acc[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = 0.0f;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-        float m = -INFINITY, l = 0.0f;
-        if (i0 + lane < parts) {
-            const float2 v = *reinterpret_cast<const float2 *>(slot(i0 + lane) + 2 * row);
-            m = v.x; l = v.y;
-        }
-        const float mine = m == -INFINITY ? 0.0f : exp2f(m - top);
-        sum += m == -INFINITY ? l : l * mine;
-        const int n = min(32, parts - i0);
-        for (int i = 0; i < n; i += 4) {
-            float x[4][N];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float *src = slot(i0 + min(i + k, n - 1)) + 2 * slot_rows + (uint64_t)row * D;
-#pragma unroll
-                for (int j = 0; j < N; ++j) x[k][j] = src[lane + 32 * j];
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float f = i + k < n ? __shfl_sync(0xffffffffu, mine, (i + k) & 31) : 0.0f;
-#pragma unroll
-                for (int j = 0; j < N; ++j) acc[j] += i + k < n ? x[k][j] * f : 0.0f;
-            }
-        }
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) top = fmaxf(top, slot(i)[2 * row]);
+    float sum = 0.0f;
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+        const float2 ml = *reinterpret_cast<const float2 *>(slot(i) + 2 * row);
+        const float4 y = *reinterpret_cast<const float4 *>(slot(i) + 2 * slot_rows + (group * slot_rows + row) * 4);
+        const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
+        sum += ml.x == -INFINITY ? ml.y : ml.y * f;
+        a.x += y.x * f; a.y += y.y * f; a.z += y.z * f; a.w += y.w * f;
     }
-    sum = warp_sum(sum);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
     const uint32_t r = (uint32_t)(sh.first_row + row);
     const uint64_t token = (uint64_t)sh.token + r / p.group, head = (uint64_t)sh.head + r % p.group;
-    T *o = reinterpret_cast<T *>(p.out) + (token * p.kv_heads * p.group + head) * D;
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const float y = acc[j] * inv;
-        bad |= !isfinite(y);
-        if constexpr (std::is_same<T, __half>::value) o[lane + 32 * j] = __float2half_rn(y);
-        else o[lane + 32 * j] = __float2bfloat16_rn(y);
-    }
-    if (bad) raise(p.status, YVEX_B200_STATUS_NUMERIC);
+    *reinterpret_cast<uint2 *>(p.out + (token * p.kv_heads * p.group + head) * D + 4 * group) = make_uint2(close2<T>(a.x, a.y), close2<T>(a.z, a.w));
+    if (!isfinite(a.x) || !isfinite(a.y) || !isfinite(a.z) || !isfinite(a.w)) raise(p.status, YVEX_B200_STATUS_NUMERIC);
 }
 
 // Which kernel, for how many rows a slot holds, on how many CTAs. Up to 16 rows fit the MMA of the rows kernel (8 with 256 dims, where
@@ -308,8 +282,8 @@ static PagedShape paged_shape(const yvex_b200_kv_cache *c, const yvex_b200_kv_st
     s.tiles = rows > (D == 256 ? 8u : 16u);
     s.rows = s.tiles ? (D == 256 ? 128u : 256u) : rows <= 8 ? 8u : 16u;
     const uint64_t keys = s.tiles ? (D == 256 ? 64u : 128u) : (uint64_t)kRowsBlock;
-    // no more CTAs than there can be blocks of keys
-    const uint64_t tiles = (rows + s.rows - 1) / s.rows, blocks = (t->longest + keys - 1) / keys;
+    // no more CTAs than there can be units of work
+    const uint64_t tiles = (rows + s.rows - 1) / s.rows, blocks = (t->longest + keys - 1) / keys + (s.tiles ? kTilesCost : kRowsCost);
     uint64_t most = (uint64_t)kSmCount * (s.tiles ? 1u : s.rows == 8 && D <= 128 ? 3u : 2u);
     for (uint64_t x : {t->requests, c->kv_heads, tiles, blocks}) if (x >= most) return s.ctas = (unsigned)most, s;
     const uint64_t bound = t->requests * c->kv_heads * tiles * blocks;
@@ -317,7 +291,7 @@ static PagedShape paged_shape(const yvex_b200_kv_cache *c, const yvex_b200_kv_st
     return s;
 }
 static uint64_t paged_partial_bytes(const PagedShape &s, uint64_t head_dim) {
-    return (2ull * s.ctas * s.rows * (head_dim + 2) * sizeof(float) + 255) / 256 * 256;
+    return (2ull * s.ctas * paged_slot_floats(s.rows, (uint32_t)head_dim) * sizeof(float) + 255) / 256 * 256;
 }
 
 template <class T, int D> static int launch_paged(const PagedParams &p, const PagedShape &s, unsigned qtype, cudaStream_t stream) {
@@ -331,7 +305,8 @@ template <class T, int D> static int launch_paged(const PagedParams &p, const Pa
         rc = ERR_BACKEND;
     }
     if (rc != OK) return rc;
-    if (launch_pdl(paged_join_kernel<T, D>, dim3(s.ctas, (s.rows + kJoinWarps - 1) / kJoinWarps), dim3(32 * kJoinWarps), 0, stream, p, (int)s.rows) != cudaSuccess)
+    const uint64_t rows = p.longest_fresh * p.group < s.rows ? p.longest_fresh * p.group : s.rows;
+    if (launch_pdl(paged_join_kernel<T, D>, dim3(s.ctas, (unsigned)((rows + kJoinRows - 1) / kJoinRows)), dim3(2 * D), 0, stream, p, (int)s.rows) != cudaSuccess)
         return ERR_BACKEND;
     return launch_status(2);
 }

@@ -2,8 +2,10 @@
 //
 // Keys and values come page by page by TMA, straight from where they lie (boxes of as many rows as a page's size allows, up to the 128
 // keys of a block), scores and the output's sums live in tensor memory, and a thread of the softmax warps owns a row, so its
-// maximum and sum need no shuffles. S = Q K^T reads both operands from shared memory; P replaces S in tensor memory, rounded once to the
-// cache's type, and is the A operand of O += P V, whose B is the V tile as it lies (N-major). Two streams of softmax warps, each with scores and
+// maximum and sum need no shuffles. S = Q K^T reads both operands from shared memory; the weights P go back to tensor memory, rounded once to
+// the cache's type, and are the A operand of O += P V, whose B is the V tile as it lies (N-major). P has columns of its own, so the buffer of S is
+// free as soon as its row is in registers and the next S is computed during the softmax (with P over S a block's chain S, softmax, PV
+// was 3960 cycles for two streams, of which the tensor cores worked 2048). Two streams of softmax warps, each with scores and
 // sums of its own, take turns with the tensor cores: with more than 128 rows they are two tiles of rows over the same keys (each block
 // of keys is read once for 256 rows); with up to 128 they are the even and the odd blocks of one tile's keys, joined when the item
 // ends. 256 columns of a head leave room for one stream (O alone takes 256 of the 512 columns of tensor memory).
@@ -27,16 +29,20 @@ template <int D> struct TilePlan {
     // registers per thread: the softmax warps hold a row of scores, the last warpgroup (copies, products) hands theirs over
     static constexpr int kLaunched = 65536 / kThreads > 255 ? 248 : 65536 / kThreads & ~7, kSoftmaxRegs = kStreams == 2 ? 208 : kLaunched, kControlRegs = kStreams == 2 ? 80 : kLaunched;
     static_assert(kSoftmaxWarps * kSoftmaxRegs + 4 * kControlRegs <= kLaunched * (kThreads / 32), "an increase would wait forever");
-    static constexpr uint32_t kOCol = kStreams == 2 ? 256 : 64;                          // columns: S of stream 0, S of stream 1, O of each
-    static constexpr uint32_t kSPitch = 128, kBadRing = 8;
+    // columns of tensor memory: the buffers of S (64 dims: one a stream; 128: one that the streams use in turn; 256: two that the stream
+    // uses in turn), then P and O of each stream
+    static constexpr uint32_t kSBuffers = D == 128 ? 1 : 2, kPCol = kSBuffers * kKeys, kOCol = kPCol + kStreams * kKeys / 2;
+    static_assert(kOCol + kStreams * D <= 512, "tensor memory has 512 columns");
+    static constexpr uint32_t kBadRing = 8, kStaging = 2048;                            // bytes of output rows that a warp turns at a time
 };
 constexpr uint32_t kTilesTmem = 512;
 
 template <int D> struct TileSmem {
     using Plan = TilePlan<D>;
-    uint64_t q_full, k_full[Plan::kStages], k_empty[Plan::kStages], v_full[Plan::kStages], v_empty[Plan::kStages];
-    uint64_t s_full[2], p_full[2], o_done[2], all, own[2], drain;
-    uint64_t scan[Plan::kThreads / 32 + 4];
+    uint4 staging[Plan::kSoftmaxWarps][Plan::kStaging / 16];
+    uint64_t q_full, q_free, k_full[Plan::kStages], k_empty[Plan::kStages], v_full[Plan::kStages], v_empty[Plan::kStages];
+    uint64_t s_full[2], s_free[2], p_full[2], o_done[2], all, own[2], drain[2];
+    PagedScratch<Plan::kThreads> scan;
     float ml[2][2][128];
     uint32_t odd[3][2][4];                       // by stream, or of both
     uint32_t bad_keys[Plan::kBadRing];
@@ -46,8 +52,22 @@ template <int D> struct TileSmem {
 
 struct TileMaps { CUtensorMap k, v; };
 
-// exp2 of a score's distance; the softmax's only transcendental
-__device__ __forceinline__ float weight_of(float x) { return exp2f(x); }
+// two sums or products in one instruction each
+__device__ __forceinline__ float2 fma2(float2 a, float b, float c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ void add2(float2 &a, float2 b) {
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a.x), "+f"(a.y) : "f"(b.x), "f"(b.y));
+}
+// 16 bytes global -> shared that complete with the thread's group of copies; zeros where `live` is false
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <class T, int D>
 __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(const __grid_constant__ TileMaps maps, const PagedParams p, const int box_keys) {
@@ -67,14 +87,17 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
     TileSmem<D> *sm = reinterpret_cast<TileSmem<D> *>(v_tiles + kStages * kTileBytes);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        mbar_init(&sm->q_full, Plan::kSoftmaxWarps);
+        mbar_init(&sm->q_full, 1);
+        mbar_init(&sm->q_free, 1);
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&sm->k_full[i], 1); mbar_init(&sm->k_empty[i], 1);
             mbar_init(&sm->v_full[i], 1); mbar_init(&sm->v_empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sm->s_full[i], 1); mbar_init(&sm->p_full[i], 4); mbar_init(&sm->o_done[i], 1); mbar_init(&sm->own[i], 4); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm->s_full[i], 1); mbar_init(&sm->s_free[i], 4); mbar_init(&sm->p_full[i], 4); mbar_init(&sm->o_done[i], 1);
+            mbar_init(&sm->own[i], 4); mbar_init(&sm->drain[i], 1);
+        }
         mbar_init(&sm->all, Plan::kSoftmaxWarps);
-        mbar_init(&sm->drain, 1);
         sm->abort = 0;
         fence_barrier_init();
     }
@@ -86,19 +109,18 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
     volatile int *abort = &sm->abort;
     pdl_trigger();
     pdl_wait();
-    const PagedStart start = paged_start<Plan::kThreads, Plan::kRows, BK>(p, sm->scan);
-    PagedWalk<Plan::kRows, BK> w;
-    w.start(p, start);
-
+    const PagedStart start = paged_start<Plan::kThreads, Plan::kRows, BK, kTilesCost>(p, &sm->scan);
     // An item of more rows than a stream has is two tiles over the same keys, otherwise the streams take turns with the blocks of keys.
-    auto rows_of = [&]() { return min(w.q.rows - w.tile * Plan::kRows, (uint32_t)Plan::kRows); };
+    using Walk = PagedWalk<Plan::kRows, BK, kTilesCost>;
+    auto rows_of = [](const Walk &w) { return min(w.q.rows - w.tile * Plan::kRows, (uint32_t)Plan::kRows); };
+    Walk w;
 
     if (warp < Plan::kSoftmaxWarps) {
         // ---------------- softmax: thread = row of a stream's tile ----------------
         set_registers<Plan::kSoftmaxRegs, Plan::kLaunched>();
         const int st = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t s_at = tmem + lanes + (uint32_t)st * Plan::kSPitch, o_at = tmem + lanes + Plan::kOCol + (uint32_t)st * D;
+        const uint32_t p_at = tmem + lanes + Plan::kPCol + (uint32_t)st * (BK / 2), o_at = tmem + lanes + Plan::kOCol + (uint32_t)st * D;
         const float scale = p.scale * 1.4426950408889634f;      // scores in powers of two
         uint32_t done = 0, all_ph = 0, own_ph = 0, odd_own = 0, odd_all = 0, it_base = 0;
         bool ok = true, bad_out = false;
@@ -115,37 +137,25 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
             ok = ok && mbar_wait_warp(&sm->own[st], own_ph, abort);
             own_ph ^= 1u;
         };
-        for (; w.live() && ok; it_base += w.count, w.next(p)) {
-            const uint32_t rows = rows_of();
+        for (w.start(p, start); w.live() && ok; it_base += w.count, w.next(p)) {
+            const uint32_t rows = rows_of(w);
             const bool two = NS == 2 && rows > 128u;            // two tiles of rows
-            const uint32_t item_row = w.tile * Plan::kRows + (two ? 128u * st : 0u) + r;
+            const uint32_t row0 = w.tile * Plan::kRows + (two ? 128u * st : 0u), item_row = row0 + r;
             const bool live = item_row < w.q.rows;
             const uint32_t token = item_row / p.group;
-            // ---- Q into shared memory, K-major with the 128-byte swizzle; one tile shared by both streams is written half by half of its dims
-            {
-                const uint16_t *src = p.q + (uint64_t)(w.q.n.token + token) * p.q_stride + ((uint64_t)w.head * p.group + item_row % p.group) * D;
-                uint8_t *dst = q_tiles + (two ? st * kQBytes : 0u);
-                const int chunks = NS == 2 && !two ? D / 16 : D / 8, c0 = NS == 2 && !two ? st * (D / 16) : 0;
-#pragma unroll 4
-                for (int i = 0; i < chunks; ++i) {
-                    const int ch = c0 + i;
-                    const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src) + ch) : make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4 *>(dst + (ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm->q_full);
-            }
-            const int64_t cached = w.q.n.cached, end = cached + w.q.n.fresh, seen = live ? cached + token + 1 : cached;
+            const int cached = (int)w.q.n.cached, end = cached + (int)w.q.n.fresh, seen = live ? cached + (int)token + 1 : cached;
             const uint64_t mask = p.tree && live ? p.ancestors[w.q.n.token + token] : 0ull;
-            const int64_t safe = p.tree ? cached : cached + (w.tile * Plan::kRows) / p.group + 1;      // keys before it are seen by every row
+            const int safe = p.tree ? cached : cached + (int)(w.tile * Plan::kRows / p.group) + 1;      // keys before it are seen by every row
             const uint32_t stride = two ? 1u : NS, begin = two ? 0u : (uint32_t)st;
             float m = -INFINITY, l = 0.0f;
             bool any = false;
             for (uint32_t j = begin; j < w.count && ok; j += stride) {
                 const uint32_t it = it_base + j;
-                const int64_t base = (int64_t)(w.first + j) * BK;
-                ok = mbar_wait_warp(&sm->s_full[st], done & 1u, abort);
+                const int base = (int)(w.first + j) * BK;
+                // (which barrier tells of S: the stream's, or with two buffers for one stream the buffer's)
+                const uint32_t full = NS == 1 ? done & 1u : (uint32_t)st, full_ph = NS == 1 ? done >> 1 : done;
+                const uint32_t buffer = Plan::kSBuffers == 1 ? 0u : full, s_at = tmem + lanes + buffer * BK;
+                ok = mbar_wait_warp(&sm->s_full[full], full_ph & 1u, abort);
                 if (!ok) break;
                 ++done;
                 tc_fence_after();
@@ -153,6 +163,9 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
 #pragma unroll
                 for (int i = 0; i < BK / 32; ++i) tmem_ld32(s_at + 32 * i, reinterpret_cast<uint32_t *>(s) + 32 * i);
                 tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm->s_free[buffer]);
                 const uint32_t bad = sm->bad_keys[it % Plan::kBadRing];      // groups of 16 keys whose page is none
                 if (base + BK > safe || bad) {
                     // ---- keys that not every row sees
@@ -177,18 +190,21 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                         const int threads = two ? 256 : 128, at = two ? tid : r;
                         if (two) odd_all ^= 1u; else odd_own ^= 1u;
                         if (at < 4) found[at] = 0u;
-                        ok = mbar_wait_warp(&sm->v_full[it % kStages], (it / kStages) & 1u, abort);
+                        // (the products of the block before have read theirs, so the tile's barrier is in this block's phase)
+                        if (any) ok = mbar_wait_warp(&sm->o_done[st], done & 1u, abort);
+                        ok = ok && mbar_wait_warp(&sm->v_full[it % kStages], (it / kStages) & 1u, abort);
                         if (two) sync_all(); else sync_own();
                         if (ok) {
                             uint8_t *tile = v_tiles + (it % kStages) * kTileBytes;
+#pragma unroll 4
                             for (int i = at; i < (int)(kTileBytes / 16); i += threads) {
                                 const int key = (i >> 3) % BK;
                                 if (base + key < cached) continue;
                                 uint4 *x = reinterpret_cast<uint4 *>(tile) + i;
-                                uint4 v = *x;
                                 if (base + key >= end) {
                                     *x = make_uint4(0, 0, 0, 0);
                                 } else {
+                                    const uint4 v = *x;
                                     const uint32_t a = odd_halves<T>(v.x), b = odd_halves<T>(v.y), c = odd_halves<T>(v.z), d = odd_halves<T>(v.w);
                                     if (a | b | c | d) {
                                         atomicOr(&found[key >> 5], 1u << (key & 31));
@@ -209,43 +225,52 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                     for (int i = 0; i < BK / 32; ++i) if (odd[i] & sees[i]) l = NAN;
                 }
                 // ---- the block's maximum; O follows it only when it must
-                float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
+                float t[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int i = 4; i < BK; i += 4) { t0 = fmaxf(t0, s[i]); t1 = fmaxf(t1, s[i + 1]); t2 = fmaxf(t2, s[i + 2]); t3 = fmaxf(t3, s[i + 3]); }
-                const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale;
+                for (int i = 4; i + 8 <= BK; i += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(t[e], s[i + e]), s[i + 4 + e]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[e] = fmaxf(t[e], s[BK - 4 + e]);
+                const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * scale;
                 float f = 1.0f;
                 if (m == -INFINITY) m = top;                    // nothing seen so far: O is zero
                 else if (top > m + kSlack) { f = exp2f(m - top); m = top; }
-                if (any && __any_sync(0xffffffffu, f != 1.0f)) {
-                    // (the scores that were just read came behind the products of the block before: O is complete)
-                    l *= f;
+                if (any) {                                      // the products of the block before: P may be written, O is complete
+                    ok = mbar_wait_warp(&sm->o_done[st], done & 1u, abort);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (__any_sync(0xffffffffu, f != 1.0f)) {
+                        l *= f;
+#pragma unroll 1
+                        for (int i = 0; i < D; i += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o_at + i, o);
+                            tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i) {
-                        uint32_t o[32];
-                        tmem_ld32(o_at + 32 * i, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st32(o_at + 32 * i, o);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st16(o_at + i, o);
+                        }
                     }
                 }
                 any = true;
-                // ---- weights, their sum, and P over S
+                // ---- weights, their sum, and P
                 const float shift = (m == -INFINITY ? 0.0f : m) - kLift;
-                float l0 = 0.0f, l1 = 0.0f;
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                for (int b = 0; b < BK / 64; ++b) {
-                    uint32_t pk[32];
+                for (int b = 0; b < BK / 32; ++b) {
+                    uint32_t pk[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float x = weight_of(fmaf(s[64 * b + 2 * i], scale, -shift)), y = weight_of(fmaf(s[64 * b + 2 * i + 1], scale, -shift));
-                        l0 += x;
-                        l1 += y;
-                        pk[i] = close2<T>(x, y);
+                    for (int i = 0; i < 16; ++i) {
+                        float2 x = fma2(make_float2(s[32 * b + 2 * i], s[32 * b + 2 * i + 1]), scale, -shift);
+                        x.x = exp2f(x.x);
+                        x.y = exp2f(x.y);
+                        add2(sum[i & 1], x);
+                        pk[i] = close2<T>(x.x, x.y);
                     }
-                    tmem_st32(s_at + 32 * b, pk);
+                    tmem_st16(p_at + 16 * b, pk);
                 }
-                l += l0 + l1;
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -280,11 +305,12 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
             const bool both = share && w.count > 1u, whole = w.begins && w.ends;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const uint32_t slot_row = item_row - w.tile * Plan::kRows;
-            float *slot = p.partial + (2ull * blockIdx.x + (w.begins ? 1 : 0)) * Plan::kRows * (D + 2);
+            float *slot = paged_slot(p, blockIdx.x, w.begins, Plan::kRows, D);
             if (!whole && live && col == 0) *reinterpret_cast<float2 *>(slot + 2 * slot_row) = make_float2(m, l);
             const uint32_t o0 = tmem + lanes + Plan::kOCol + (two ? (uint32_t)st * D : 0u);
-            uint16_t *out = p.out + ((uint64_t)(w.q.n.token + token) * p.kv_heads * p.group + (uint64_t)w.head * p.group + item_row % p.group) * D;
-            float *part = slot + 2 * Plan::kRows + (uint64_t)slot_row * D;
+            const uint64_t heads = (uint64_t)p.kv_heads * p.group;
+            uint4 *turn = sm->staging[warp];
+#pragma unroll 1
             for (uint32_t c = col; c < col + cols; c += 32) {
                 uint32_t a[32];
                 tmem_ld32(o0 + c, a);
@@ -301,52 +327,65 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                         for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) * f0);
                     }
                 }
-                if (!live) continue;
                 if (whole) {
+                    // 32 rows x 64 bytes turned in shared memory, so that four lanes write a row's 64 bytes instead of one lane its 16
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
+                    for (int e = 0; e < 4; ++e) {
                         uint32_t o[4];
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            const float y0 = __uint_as_float(a[e + 2 * x]) * inv, y1 = __uint_as_float(a[e + 2 * x + 1]) * inv;
-                            bad_out |= !isfinite(y0) || !isfinite(y1);
+                            const float y0 = __uint_as_float(a[8 * e + 2 * x]) * inv, y1 = __uint_as_float(a[8 * e + 2 * x + 1]) * inv;
+                            bad_out |= live && (!isfinite(y0) || !isfinite(y1));
                             o[x] = close2<T>(y0, y1);
                         }
-                        *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(o[0], o[1], o[2], o[3]);
+                        turn[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_uint4(o[0], o[1], o[2], o[3]);
                     }
-                } else {
+                    __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) *reinterpret_cast<float2 *>(part + c + e) = make_float2(__uint_as_float(a[e]), __uint_as_float(a[e + 1]));
+                    for (int e = 0; e < 4; ++e) {
+                        const int q = 8 * e + (lane >> 2);
+                        const uint32_t row = row0 + 32u * (warp & 3) + q;
+                        const uint4 x = turn[q * 4 + ((lane & 3) ^ ((q >> 1) & 3))];
+                        if (row < w.q.rows)
+                            *reinterpret_cast<uint4 *>(p.out + ((w.q.n.token + row / p.group) * heads + (uint64_t)w.head * p.group + row % p.group) * D + c + 8 * (lane & 3)) = x;
+                    }
+                    __syncwarp();
+                } else if (live) {
+                    float4 *part = reinterpret_cast<float4 *>(slot + 2 * Plan::kRows) + (uint64_t)(c / 4) * Plan::kRows + slot_row;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        part[e * Plan::kRows] = make_float4(__uint_as_float(a[4 * e]), __uint_as_float(a[4 * e + 1]), __uint_as_float(a[4 * e + 2]), __uint_as_float(a[4 * e + 3]));
                 }
             }
             if (tid == 0 && w.begins && !w.ends)
                 p.share[blockIdx.x] = PagedShare{w.last_cta(start), (int32_t)rows, (int32_t)w.q.n.token, (int32_t)(w.head * p.group),
                                                  (int32_t)(w.tile * Plan::kRows), {0, 0, 0}};
-            tc_fence_before();
-            sync_all();                                         // Q and the sums may be written again
-            tc_fence_after();
+            if (share) {                                        // either stream's sums may be written again
+                tc_fence_before();
+                sync_all();
+            }
         }
         if (bad_out) raise(p.status, YVEX_B200_STATUS_NUMERIC);
     } else {
     set_registers<Plan::kControlRegs, Plan::kLaunched>();
+    w.start(p, start);
     if (warp == Plan::kSoftmaxWarps) {
         // ---------------- TMA producer: a lane per box of a block ----------------
         const int boxes = BK / box_keys;
         const uint32_t nowhere = (uint32_t)(p.pages * p.kv_heads * p.page_size);      // a row past the cache: the box is filled with zeros
         const uint32_t groups = (uint32_t)box_keys / 16u, page_size = (uint32_t)p.page_size;
         bool ok = true, bad_page = false;
-        uint32_t it = 0;
+        uint32_t it = 0, k_asked = 0;
         for (; w.live() && ok; w.next(p)) {
-            const int64_t end = (int64_t)w.q.n.cached + w.q.n.fresh;
+            const uint32_t end = w.q.n.cached + w.q.n.fresh;
             const int32_t *table = p.block_table + (uint64_t)w.request * p.table_width;
             auto row_of = [&](uint32_t j, bool &none) -> uint32_t {      // where this lane's box of block j begins; none: no page holds it
                 none = false;
-                if (lane >= boxes || j >= w.count) return nowhere;
-                const int64_t key = (int64_t)(w.first + j) * BK + (int64_t)lane * box_keys;
-                if (key >= end) return nowhere;
-                const int32_t page = __ldg(table + (uint32_t)key / page_size);
+                const uint32_t key = (w.first + j) * BK + (uint32_t)(lane * box_keys);
+                if (lane >= boxes || j >= w.count || key >= end) return nowhere;
+                const int32_t page = __ldg(table + key / page_size);
                 none = page < 0 || (uint64_t)page >= p.pages;
-                return none ? nowhere : ((uint32_t)page * p.kv_heads + w.head) * page_size + (uint32_t)key % page_size;
+                return none ? nowhere : ((uint32_t)page * p.kv_heads + w.head) * page_size + key % page_size;
             };
             bool none, none_next;
             uint32_t y = row_of(0, none);
@@ -361,6 +400,7 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                 if (lane < boxes)
                     for (int h = 0; h < kHalves; ++h)
                         tma_load_2d(k_tiles + s * kTileBytes + h * BK * 128 + lane * box_keys * 128, &maps.k, 64 * h, (int)y, &sm->k_full[s]);
+                k_asked = it + 1;
                 ok = mbar_wait_warp(&sm->v_empty[s], ph ^ 1u, abort);
                 if (!ok) break;
                 if (lane == 0) mbar_expect_tx(&sm->v_full[s], kTileBytes);
@@ -376,79 +416,108 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
         if (!ok && lane == 0) {
             // copies in flight must land before the CTA's shared memory is someone else's
             volatile int none = 0;
-            for (uint32_t i = it >= kStages ? it - kStages : 0; i < it; ++i) {
-                mbar_wait(&sm->k_full[i % kStages], (i / kStages) & 1u, &none);
-                mbar_wait(&sm->v_full[i % kStages], (i / kStages) & 1u, &none);
-            }
-            mbar_wait(&sm->k_full[it % kStages], (it / kStages) & 1u, &none, 1000000ull);      // (a K tile whose V was not asked for)
+            for (uint32_t i = k_asked > kStages ? k_asked - kStages : 0; i < k_asked; ++i) mbar_wait(&sm->k_full[i % kStages], (i / kStages) & 1u, &none);
+            for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_wait(&sm->v_full[i % kStages], (i / kStages) & 1u, &none);
         }
         __syncwarp();
-    } else if (warp == Plan::kSoftmaxWarps + 1 && elect_one()) {
-        // ---------------- MMA issuer: whichever stream is ready ----------------
-        constexpr uint32_t kIdescS = idesc_16bit(!kHalfType, false, BK), kIdescO = idesc_16bit(!kHalfType, true, D);
-        const uint64_t q0 = smem_desc_sw128(smem_u32(q_tiles)), k0 = smem_desc_sw128(smem_u32(k_tiles));
-        const uint64_t v0 = smem_desc_n_major_sw128(smem_u32(v_tiles), BK * 128);
-        uint32_t it_base = 0, segment = 0, asked[2] = {0, 0}, given[2] = {0, 0};      // S and PV issued per stream so far
-        bool ok = true;
-        for (; w.live() && ok; it_base += w.count, w.next(p), ++segment) {
-            const bool two = NS == 2 && rows_of() > 128u;
-            ok = mbar_wait(&sm->q_full, segment & 1u, abort);
-            if (!ok) break;
-            uint32_t n[2], s_i[2] = {0, 0}, v_i[2] = {0, 0};
-            n[0] = two || NS == 1 ? w.count : (w.count + 1) / 2;
-            n[1] = NS == 1 ? 0 : two ? w.count : w.count / 2;
-            const uint32_t stride = two || NS == 1 ? 1u : 2u;
-            uint64_t t0 = 0;
-            uint32_t idle = 0;
-            while (v_i[0] < n[0] || v_i[1] < n[1]) {
-                bool moved = false;
+    } else if (warp == Plan::kSoftmaxWarps + 1) {
+        // ---------------- S = Q K^T, block after block and stream after stream; one lane issues ----------------
+        if (elect_one()) {
+            constexpr uint32_t kIdesc = idesc_16bit(!kHalfType, false, BK);
+            const uint64_t q0 = smem_desc_sw128(smem_u32(q_tiles)), k0 = smem_desc_sw128(smem_u32(k_tiles));
+            uint32_t it = 0, segment = 0, used = 0, asked[2] = {0, 0};      // blocks, segments, S so far, S of a stream
+            bool ok = true;
+            for (; w.live() && ok; w.next(p), ++segment) {
+                const bool two = NS == 2 && rows_of(w) > 128u;
+                ok = mbar_wait(&sm->q_full, segment & 1u, abort);
+                for (uint32_t j = 0; j < w.count && ok; ++j, ++it) {
+                    const uint32_t s = it % kStages;
+                    const uint64_t kd = k0 + s * (kTileBytes >> 4);
+                    ok = mbar_wait(&sm->k_full[s], (it / kStages) & 1u, abort);
 #pragma unroll
-                for (int st = 0; st < NS; ++st) {
-                    if (s_i[st] == v_i[st]) {
-                        if (s_i[st] == n[st]) continue;
-                        // S of the stream's next block: its P of the block before has been used, the keys are there
-                        const uint32_t it = it_base + (two ? s_i[st] : s_i[st] * stride + st), s = it % kStages;
-                        if (given[st] && !mbar_try_wait(&sm->o_done[st], (given[st] - 1u) & 1u)) continue;
-                        if (!mbar_try_wait(&sm->k_full[s], (it / kStages) & 1u)) continue;
+                    for (uint32_t st = 0; st < NS; ++st) {
+                        if (!ok || (!two && NS == 2 && (j & 1u) != st)) continue;
+                        const uint32_t n = asked[st]++, full = NS == 1 ? n & 1u : st, b = Plan::kSBuffers == 1 ? 0u : full;
+                        // the buffer has been read since it was last used (every phase of a barrier is waited for in turn: parities tell no more)
+                        const uint32_t uses = Plan::kSBuffers == 1 ? used : NS == 1 ? n >> 1 : n;
+                        if (uses) ok = mbar_wait(&sm->s_free[b], (uses - 1u) & 1u, abort);
+                        if (!ok) continue;
+                        ++used;
                         tc_fence_after();
-                        const uint64_t qd = q0 + (two ? st * (kQBytes >> 4) : 0u), kd = k0 + s * (kTileBytes >> 4);
+                        const uint64_t qd = q0 + (two ? st * (kQBytes >> 4) : 0u);
 #pragma unroll
                         for (int k = 0; k < D / 16; ++k)
-                            umma_f16(tmem + st * Plan::kSPitch, qd + (k >> 2) * (16384 >> 4) + 2 * (k & 3), kd + (k >> 2) * (BK * 128 >> 4) + 2 * (k & 3), kIdescS, k ? 1u : 0u);
-                        umma_commit(&sm->s_full[st]);
-                        ++s_i[st];
-                        ++asked[st];
-                        if (!two || s_i[st ^ 1] >= s_i[st]) umma_commit(&sm->k_empty[s]);
-                        moved = true;
-                    } else {
-                        // O += P V of the stream's block
-                        const uint32_t it = it_base + (two ? v_i[st] : v_i[st] * stride + st), s = it % kStages;
-                        if (!mbar_try_wait(&sm->p_full[st], (asked[st] - 1u) & 1u) || !mbar_try_wait(&sm->v_full[s], (it / kStages) & 1u)) continue;
-                        tc_fence_after();
-                        const uint64_t vd = v0 + s * (kTileBytes >> 4);
-#pragma unroll
-                        for (int k = 0; k < BK / 16; ++k)
-                            umma_f16_ts(tmem + Plan::kOCol + st * D, tmem + st * Plan::kSPitch + 8 * k, vd + k * (2048 >> 4), kIdescO, v_i[st] | k ? 1u : 0u);
-                        umma_commit(&sm->o_done[st]);
-                        ++v_i[st];
-                        ++given[st];
-                        if (!two || v_i[st ^ 1] >= v_i[st]) umma_commit(&sm->v_empty[s]);
-                        moved = true;
+                            umma_f16(tmem + b * BK, qd + (k >> 2) * (16384 >> 4) + 2 * (k & 3), kd + (k >> 2) * (BK * 128 >> 4) + 2 * (k & 3), kIdesc, k ? 1u : 0u);
+                        umma_commit(&sm->s_full[full]);
                     }
+                    if (ok) umma_commit(&sm->k_empty[s]);
                 }
-                if (moved) { idle = 0; t0 = 0; continue; }
-                if ((++idle & 63u) == 0u) {                     // bounded like every wait
-                    const uint64_t now = global_ns();
-                    if (*abort || (t0 && now - t0 > kWaitLimitNs)) { *abort = 1; ok = false; break; }
-                    if (!t0) t0 = now;
-                }
+                if (ok) umma_commit(&sm->q_free);
+            }
+            if (!ok) {
+                volatile int none = 0;
+                umma_commit(&sm->drain[0]);                     // products in flight end before the tensor memory is freed
+                mbar_wait(&sm->drain[0], 0u, &none);
             }
         }
-        if (!ok) {
-            volatile int none = 0;
-            umma_commit(&sm->drain);                            // products in flight end before the tensor memory is freed
-            mbar_wait(&sm->drain, 0u, &none);
+    } else if (warp == Plan::kSoftmaxWarps + 2) {
+        // ---------------- O += P V in the same order, behind the softmax; one lane issues ----------------
+        if (elect_one()) {
+            constexpr uint32_t kIdesc = idesc_16bit(!kHalfType, true, D);
+            const uint64_t v0 = smem_desc_n_major_sw128(smem_u32(v_tiles), BK * 128);
+            uint32_t it = 0, given[2] = {0, 0};
+            bool ok = true;
+            for (; w.live() && ok; w.next(p)) {
+                const bool two = NS == 2 && rows_of(w) > 128u;
+                for (uint32_t j = 0; j < w.count && ok; ++j, ++it) {
+                    const uint32_t s = it % kStages;
+                    const uint64_t vd = v0 + s * (kTileBytes >> 4);
+                    ok = mbar_wait(&sm->v_full[s], (it / kStages) & 1u, abort);
+#pragma unroll
+                    for (uint32_t st = 0; st < NS; ++st) {
+                        if (!ok || (!two && NS == 2 && (j & 1u) != st)) continue;
+                        ok = mbar_wait(&sm->p_full[st], given[st] & 1u, abort);
+                        if (!ok) continue;
+                        ++given[st];
+                        tc_fence_after();
+                        const uint32_t first = two || NS == 1 ? j : j >> 1;      // 0: the sums begin
+#pragma unroll
+                        for (int k = 0; k < BK / 16; ++k)
+                            umma_f16_ts(tmem + Plan::kOCol + st * D, tmem + Plan::kPCol + st * (BK / 2) + 8 * k, vd + k * (2048 >> 4), kIdesc, first || k ? 1u : 0u);
+                        umma_commit(&sm->o_done[st]);
+                    }
+                    if (ok) umma_commit(&sm->v_empty[s]);
+                }
+            }
+            if (!ok) {
+                volatile int none = 0;
+                umma_commit(&sm->drain[1]);
+                mbar_wait(&sm->drain[1], 0u, &none);
+            }
         }
+    } else if (warp == Plan::kSoftmaxWarps + 3) {
+        // ---------------- Q: rows of an item while the one before is being finished, K-major with the 128-byte swizzle ----------------
+        constexpr int kLanes = D / 8, kAt = 32 / kLanes;         // lanes of a row, rows at a time
+        const uint32_t chunk = (uint32_t)lane % kLanes;
+        bool ok = true;
+        for (uint32_t segment = 0; w.live() && ok; w.next(p), ++segment) {
+            if (segment) ok = mbar_wait_warp(&sm->q_free, (segment - 1u) & 1u, abort);
+            if (!ok) break;
+            const uint32_t rows = rows_of(w), tiles = NS == 2 && rows > 128u ? 2u : 1u;
+#pragma unroll 4
+            for (uint32_t row = (uint32_t)lane / kLanes; row < 128u * tiles; row += kAt) {
+                const bool live = row < rows;
+                const uint32_t at = live ? w.tile * Plan::kRows + row : 0u, token = at / p.group;
+                const uint16_t *src = p.q + (uint64_t)(w.q.n.token + token) * p.q_stride + ((uint64_t)w.head * p.group + at % p.group) * D + 8 * chunk;
+                const uint32_t rr = row & 127u;
+                copy16(q_tiles + (row >> 7) * kQBytes + (chunk >> 3) * 16384 + rr * 128 + (((chunk & 7u) ^ (rr & 7u)) << 4), src, live);
+            }
+            copies_done();
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm->q_full);
+        }
+        copies_done();
     }
     }
     tc_fence_before();

@@ -22,9 +22,11 @@ struct PagedParams {
     const uint64_t *ancestors;
     float scale;
     int *status;
-    float *partial;                              // [2 * CTAs] slots of rows x (maximum, sum), then rows x head_dim
+    float *partial;                              // [2 * CTAs] slots
     struct PagedShare *share;                    // [CTAs]
 };
+
+constexpr int kTilesCost = 2;                    // of the tiles kernel, in its blocks of 128 keys (64 with 256 dims)
 
 // An item that a CTA began: CTAs c .. last hold its parts. rows 0: none.
 struct PagedShare { int32_t last, rows, token, head, first_row, pad[3]; };
@@ -51,119 +53,165 @@ __device__ __forceinline__ uint32_t paged_visible(const PagedParams &p, const Pa
 template <int MROWS, int BK> struct PagedRequest {
     PagedLengths n;
     uint32_t rows, tiles;
-    __device__ void open(const PagedParams &p, uint64_t r) {
+    __device__ __forceinline__ void open(const PagedParams &p, uint64_t r) {
         n = paged_lengths(p, r);
         rows = n.fresh * p.group;
         tiles = (rows + MROWS - 1) / MROWS;
     }
-    __device__ uint32_t blocks(const PagedParams &p, uint32_t tile) const {
+    __device__ __forceinline__ uint32_t blocks(const PagedParams &p, uint32_t tile) const {
         return (paged_visible(p, n, min(rows, (tile + 1u) * MROWS)) + BK - 1) / BK;
-    }
-    __device__ uint64_t blocks_per_head(const PagedParams &p) const {
-        if (p.tree || tiles <= 1u) return tiles ? (uint64_t)tiles * blocks(p, 0) : 0ull;
-        uint64_t sum = 0;
-        for (uint32_t t = 0; t < tiles; ++t) sum += blocks(p, t);
-        return sum;
     }
 };
 
-// Where a CTA's share begins, found by all its threads (NT of them; `scratch`: NT / 32 + 4 words of shared memory).
-struct PagedStart { uint64_t total, from, left, skip; uint32_t request, ctas; };
-template <int NT, int MROWS, int BK>
-__device__ PagedStart paged_start(const PagedParams &p, uint64_t *scratch) {
+// Where a CTA's share begins, found by all its threads (NT of them). COST: what beginning and ending an item costs, in blocks; they
+// stand before the item's first block when the shares are cut.
+struct PagedStart { uint64_t total, from, left; uint32_t request, head, tile, skip, ctas; };
+template <int NT> struct PagedScratch {
+    uint64_t warps[NT / 32], sum, skip;
+    uint32_t request, head, tile, first;
+    uint64_t units[NT / 8];
+};
+template <int NT, int MROWS, int BK, int COST>
+__device__ PagedStart paged_start(const PagedParams &p, PagedScratch<NT> *sc) {
     constexpr int W = NT / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto units = [&](uint64_t r) -> uint64_t {
+    using Request = PagedRequest<MROWS, BK>;
+    auto tile_units = [&](const Request &q, uint32_t t) { return t < q.tiles ? q.blocks(p, t) + COST : 0u; };
+    auto units = [&](uint64_t r) -> uint64_t {                  // of one request and kv head, by one thread
         if (r >= p.requests) return 0;
-        PagedRequest<MROWS, BK> q;
+        Request q;
         q.open(p, r);
         if (q.n.bad && blockIdx.x == 0) raise(p.status, YVEX_B200_STATUS_ARGUMENT);
-        return q.blocks_per_head(p) * p.kv_heads;
+        if (p.tree) return (uint64_t)q.tiles * tile_units(q, 0);
+        uint64_t sum = 0;
+        for (uint32_t t = 0; t < q.tiles; ++t) sum += tile_units(q, t);
+        return sum;
     };
-    auto sum_warps = [&](uint64_t v) {                          // inclusive prefix over the block's threads; the sum in scratch[W]
+    auto scan = [&](uint64_t v) {                               // inclusive prefix over the block's threads; the sum in sc->sum
         uint64_t s = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t a = __shfl_up_sync(0xffffffffu, s, o);
             if (lane >= o) s += a;
         }
-        if (lane == 31) scratch[warp] = s;
+        if (lane == 31) sc->warps[warp] = s;
         __syncthreads();
         uint64_t before = 0, all = 0;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            if (w < warp) before += scratch[w];
-            all += scratch[w];
+            if (w < warp) before += sc->warps[w];
+            all += sc->warps[w];
         }
-        if (tid == 0) scratch[W] = all;
+        if (tid == 0) sc->sum = all;
+        __syncthreads();
         return s + before;
     };
     PagedStart st;
-    const bool single = p.requests <= NT;                       // one request a thread
-    const uint64_t first = units((uint64_t)tid);
+    // A few requests of many tiles (a prompt) are counted by a warp each, many requests by a thread each.
+    const bool few = !p.tree && p.longest_fresh * p.group > (uint64_t)MROWS && p.requests <= NT / 8, single = p.requests <= NT;
+    uint64_t first;
+    if (few) {
+        for (uint32_t r = warp; r < (uint32_t)p.requests; r += W) {
+            Request q;
+            q.open(p, r);
+            if (q.n.bad && blockIdx.x == 0 && lane == 0) raise(p.status, YVEX_B200_STATUS_ARGUMENT);
+            uint64_t sum = 0;
+            for (uint32_t t = lane; t < q.tiles; t += 32) sum += tile_units(q, t);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) sc->units[r] = sum;
+        }
+        __syncthreads();
+        first = tid < (int)p.requests ? sc->units[tid] : 0;
+    } else {
+        first = units((uint64_t)tid);
+    }
     uint64_t v = first;
     if (!single)
         for (uint64_t r = (uint64_t)tid + NT; r < p.requests; r += NT) v += units(r);
-    uint64_t prefix = sum_warps(v);
-    __syncthreads();
-    st.total = scratch[W];
-    st.ctas = (uint32_t)min((uint64_t)gridDim.x, st.total);     // every CTA that has a share has a block at least
+    uint64_t prefix = scan(v);
+    st.total = sc->sum * p.kv_heads;
+    st.ctas = (uint32_t)min((uint64_t)gridDim.x, st.total);     // every CTA that has a share has a unit at least
     const uint64_t u0 = blockIdx.x < st.ctas ? st.total * blockIdx.x / st.ctas : st.total;
     const uint64_t u1 = blockIdx.x < st.ctas ? st.total * (blockIdx.x + 1ull) / st.ctas : st.total;
     st.from = u0;
     st.left = u1 - u0;
     uint64_t base = 0;
-    for (uint64_t chunk = 0; chunk < p.requests; chunk += NT) {
+    for (uint64_t chunk = 0; chunk < p.requests && st.left; chunk += NT) {
         if (!single) {
             __syncthreads();
             v = chunk ? units(chunk + tid) : first;
-            prefix = sum_warps(v);
-            __syncthreads();
+            prefix = scan(v);
         }
-        const uint64_t begin = base + prefix - v;
-        if (v && u0 >= begin && u0 < begin + v) { scratch[W + 1] = chunk + tid; scratch[W + 2] = u0 - begin; }
-        base += scratch[W];
-        if (base > u0) break;
+        const uint64_t begin = (base + prefix - v) * p.kv_heads;
+        if (v && u0 >= begin && u0 < begin + v * p.kv_heads) {
+            const uint64_t skip = u0 - begin, head = skip / v;
+            sc->request = (uint32_t)(chunk + tid);
+            sc->head = (uint32_t)head;
+            sc->skip = skip - head * v;
+        }
+        base += sc->sum;
+        if (base * p.kv_heads > u0) break;
     }
     __syncthreads();
-    st.request = st.left ? (uint32_t)scratch[W + 1] : 0u;
-    st.skip = st.left ? scratch[W + 2] : 0ull;
+    if (warp == 0 && st.left) {                                 // the tile of that request: the first whose units reach past what is skipped
+        Request q;
+        q.open(p, sc->request);
+        uint64_t skip = sc->skip;
+        for (uint32_t t0 = 0; t0 < q.tiles; t0 += 32) {
+            const uint32_t mine = tile_units(q, t0 + lane);
+            uint64_t s = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t a = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += a;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, s > skip);
+            if (past) {
+                if (lane == __ffs((int)past) - 1) { sc->tile = t0 + lane; sc->first = (uint32_t)(skip - (s - mine)); }
+                break;
+            }
+            skip -= __shfl_sync(0xffffffffu, s, 31);
+        }
+    }
     __syncthreads();
+    st.request = sc->request;
+    st.head = sc->head;
+    st.tile = sc->tile;
+    st.skip = sc->first;
     return st;
 }
 
 // The segments of a CTA's share, one after the other; every role of a CTA walks them by itself.
-template <int MROWS, int BK> struct PagedWalk {
+template <int MROWS, int BK, int COST> struct PagedWalk {
     PagedRequest<MROWS, BK> q;
-    uint64_t left, at;                           // blocks of the share still to come; place of the next one among all blocks
-    uint32_t request, head, tile, first, count, blocks;
+    uint64_t left, at;                           // units of the share still to come; place of the next one among all units
+    uint32_t request, head, tile, first, count, blocks, rest;
     bool begins, ends;                           // the segment holds the item's first block, its last
-    __device__ void start(const PagedParams &p, const PagedStart &s) {
+    __device__ __forceinline__ void start(const PagedParams &p, const PagedStart &s) {
         left = s.left;
         at = s.from;
         request = s.request;
+        head = s.head;
+        tile = s.tile;
         count = 0;
         if (!left) return;
         q.open(p, request);
-        const uint64_t per_head = q.blocks_per_head(p);
-        uint64_t skip = s.skip;
-        head = (uint32_t)(skip / per_head);
-        skip -= head * per_head;
-        tile = 0;
-        if (p.tree) { blocks = q.blocks(p, 0); tile = (uint32_t)(skip / blocks); skip -= (uint64_t)tile * blocks; }
-        else for (; (blocks = q.blocks(p, tile)) <= skip; ++tile) skip -= blocks;
-        first = (uint32_t)skip;
-        cut();
+        cut(p, s.skip);
     }
-    __device__ void cut() {
-        count = (uint32_t)min((uint64_t)(blocks - first), left);
+    __device__ __forceinline__ void cut(const PagedParams &p, uint32_t from) {
+        blocks = q.blocks(p, tile);
+        const uint32_t to = (uint32_t)min((uint64_t)(blocks + COST), from + left), units = to - from;
+        first = from > COST ? from - COST : 0u;
+        count = (to > COST ? to - COST : 0u) - first;           // 0 only where the share ends within the cost of an item's beginning
         begins = first == 0;
         ends = first + count == blocks;
-        left -= count;
-        at += count;
+        rest = blocks + COST - to;
+        left -= units;
+        at += units;
     }
-    __device__ bool live() const { return count != 0; }
-    __device__ void next(const PagedParams &p) {
+    __device__ __forceinline__ bool live() const { return count != 0; }
+    __device__ __forceinline__ void next(const PagedParams &p) {
         count = 0;
         if (!left) return;
         if (++tile == q.tiles) {
@@ -173,16 +221,18 @@ template <int MROWS, int BK> struct PagedWalk {
                 do q.open(p, ++request); while (q.rows == 0);   // (there is work left, so there is such a request)
             }
         }
-        blocks = q.blocks(p, tile);
-        first = 0;
-        cut();
+        cut(p, 0);
     }
     // The CTA that holds the item's last block; of a segment that does not end its item.
-    __device__ int32_t last_cta(const PagedStart &s) const {
-        const uint64_t u = at + (blocks - first - count) - 1;   // `at` is behind the segment
-        return (int32_t)(((u + 1) * s.ctas - 1) / s.total);
-    }
+    __device__ __forceinline__ int32_t last_cta(const PagedStart &s) const { return (int32_t)(((at + rest) * s.ctas - 1) / s.total); }
 };
+
+// A slot of the workspace: (maximum, sum) of every row, then the accumulators in groups of four columns, [head_dim / 4][rows][4], so that
+// threads with a row each write whole lines.
+__host__ __device__ constexpr uint64_t paged_slot_floats(uint32_t rows, uint32_t head_dim) { return (uint64_t)rows * (head_dim + 2); }
+__device__ __forceinline__ float *paged_slot(const PagedParams &p, uint32_t cta, bool began, uint32_t rows, uint32_t head_dim) {
+    return p.partial + (2ull * cta + (began ? 1 : 0)) * paged_slot_floats(rows, head_dim);
+}
 
 // Which of the keys base .. base + 63 a row sees, as bits. chain: keys below `seen`; tree: keys below `cached`, and of those from
 // there on (base may lie before or behind) the bits of `mask`.
