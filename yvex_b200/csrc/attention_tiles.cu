@@ -41,16 +41,23 @@ template <int D> struct TileSmem {
     using Plan = TilePlan<D>;
     uint4 staging[Plan::kSoftmaxWarps][Plan::kStaging / 16];
     uint64_t q_full, q_free, k_full[Plan::kStages], k_empty[Plan::kStages], v_full[Plan::kStages], v_empty[Plan::kStages];
-    uint64_t s_full[2], s_free[2], p_full[2], o_done[2], all, own[2], drain[2];
+    uint64_t s_full[2], s_free[2], p_full[2], o_done[2], v_clean[Plan::kStages], all, looked, noted, drain[2];
     PagedScratch<Plan::kThreads> scan;
     float ml[2][2][128];
-    uint32_t odd[3][2][4];                       // by stream, or of both
+    unsigned long long odd_mask;                 // the item's fresh tokens with values that are not finite: as bits, and the first of them
+    int odd_first;
     uint32_t bad_keys[Plan::kBadRing];
     uint32_t tmem_base;
     int abort;
 };
 
-struct TileMaps { CUtensorMap k, v; };
+// q: rows of Q as {head_dim, query heads, tokens}, boxes of 64 values x a group x 128 / group tokens
+struct TileMaps { CUtensorMap k, v, q; };
+
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(sm100::smem_u32(dst)), "l"(map), "r"(sm100::smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
 
 // two sums or products in one instruction each
 __device__ __forceinline__ float2 fma2(float2 a, float b, float c) {
@@ -63,6 +70,9 @@ __device__ __forceinline__ void add2(float2 &a, float2 b) {
     asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
         : "+f"(a.x), "+f"(a.y) : "f"(b.x), "f"(b.y));
 }
+template <class T> struct PairOf { using type = __half2; };
+template <> struct PairOf<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <class T> __device__ __forceinline__ typename PairOf<T>::type pair_of(uint32_t w) { return *reinterpret_cast<typename PairOf<T>::type *>(&w); }
 // 16 bytes global -> shared that complete with the thread's group of copies; zeros where `live` is false
 __device__ __forceinline__ void copy16(void *dst, const void *src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(live ? 16 : 0) : "memory");
@@ -70,7 +80,7 @@ __device__ __forceinline__ void copy16(void *dst, const void *src, bool live) {
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <class T, int D>
-__global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(const __grid_constant__ TileMaps maps, const PagedParams p, const int box_keys) {
+__global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(const __grid_constant__ TileMaps maps, const PagedParams p, const int box_keys, const int q_tokens) {
     using namespace sm100;
     using Plan = TilePlan<D>;
     constexpr int BK = Plan::kKeys, NS = Plan::kStreams, kStages = Plan::kStages, kHalves = D / 64;
@@ -91,13 +101,15 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
         mbar_init(&sm->q_free, 1);
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&sm->k_full[i], 1); mbar_init(&sm->k_empty[i], 1);
-            mbar_init(&sm->v_full[i], 1); mbar_init(&sm->v_empty[i], 1);
+            mbar_init(&sm->v_full[i], 1); mbar_init(&sm->v_empty[i], 2); mbar_init(&sm->v_clean[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm->s_full[i], 1); mbar_init(&sm->s_free[i], 4); mbar_init(&sm->p_full[i], 4); mbar_init(&sm->o_done[i], 1);
-            mbar_init(&sm->own[i], 4); mbar_init(&sm->drain[i], 1);
+            mbar_init(&sm->drain[i], 1);
         }
         mbar_init(&sm->all, Plan::kSoftmaxWarps);
+        mbar_init(&sm->looked, 1);
+        mbar_init(&sm->noted, Plan::kSoftmaxWarps);
         sm->abort = 0;
         fence_barrier_init();
     }
@@ -112,8 +124,36 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
     const PagedStart start = paged_start<Plan::kThreads, Plan::kRows, BK, kTilesCost>(p, &sm->scan);
     // An item of more rows than a stream has is two tiles over the same keys, otherwise the streams take turns with the blocks of keys.
     using Walk = PagedWalk<Plan::kRows, BK, kTilesCost>;
+    // ..., and the keys before this one are seen by every row.
+    auto safe_keys = [&](const Walk &w) { return (int)w.q.n.cached + (p.tree ? 0 : (int)(w.tile * Plan::kRows / p.group) + 1); };
     auto rows_of = [](const Walk &w) { return min(w.q.rows - w.tile * Plan::kRows, (uint32_t)Plan::kRows); };
     Walk w;
+
+    // Q of an item into shared memory, K-major with the 128-byte swizzle. Where a tile's 128 rows are whole tokens (q_tokens of them) it is
+    // a box per 64 dims; the rows behind the item's last one are then some other rows, whose results go nowhere.
+    auto load_q = [&]() {                                       // by one lane
+        const uint32_t tiles = NS == 2 && rows_of(w) > 128u ? 2u : 1u;
+        mbar_expect_tx(&sm->q_full, tiles * kQBytes);
+        for (uint32_t t = 0; t < tiles; ++t)
+            for (int h = 0; h < kHalves; ++h)
+                tma_load_3d(q_tiles + t * kQBytes + h * 16384, &maps.q, 64 * h, (int)(w.head * p.group),
+                            (int)(w.q.n.token + (w.tile * (Plan::kRows / 128) + t) * (uint32_t)q_tokens), &sm->q_full);
+    };
+    // Other groups' rows are copied one by one, by some warps; the copies are complete on return.
+    auto copy_q = [&](uint32_t first, uint32_t step) {
+        constexpr uint32_t kLanes = D / 8, kAt = 32 / kLanes;    // lanes of a row, rows at a time
+        const uint32_t chunk = (uint32_t)lane % kLanes, rows = rows_of(w), end = NS == 2 && rows > 128u ? 256u : 128u;
+        const uint16_t *src = p.q + (uint64_t)w.head * p.group * D + 8 * chunk;
+#pragma unroll 4
+        for (uint32_t row = first * kAt + (uint32_t)lane / kLanes; row < end; row += step * kAt) {
+            const bool live = row < rows;
+            const uint32_t at = live ? w.tile * Plan::kRows + row : 0u, token = at / p.group, rr = row & 127u;
+            copy16(q_tiles + (row >> 7) * kQBytes + (chunk >> 3) * 16384 + rr * 128 + (((chunk & 7u) ^ (rr & 7u)) << 4),
+                   src + (uint64_t)(w.q.n.token + token) * p.q_stride + (uint64_t)(at - token * p.group) * D, live);
+        }
+        copies_done();
+        fence_proxy_async();
+    };
 
     if (warp < Plan::kSoftmaxWarps) {
         // ---------------- softmax: thread = row of a stream's tile ----------------
@@ -122,7 +162,7 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t p_at = tmem + lanes + Plan::kPCol + (uint32_t)st * (BK / 2), o_at = tmem + lanes + Plan::kOCol + (uint32_t)st * D;
         const float scale = p.scale * 1.4426950408889634f;      // scores in powers of two
-        uint32_t done = 0, all_ph = 0, own_ph = 0, odd_own = 0, odd_all = 0, it_base = 0;
+        uint32_t done = 0, all_ph = 0, it_base = 0, segment = 0;
         bool ok = true, bad_out = false;
         if (tid == 0) p.share[blockIdx.x].rows = 0;
         auto sync_all = [&]() {                                 // every softmax thread of the CTA; bounded like every wait
@@ -131,13 +171,13 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
             ok = ok && mbar_wait_warp(&sm->all, all_ph, abort);
             all_ph ^= 1u;
         };
-        auto sync_own = [&]() {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm->own[st]);
-            ok = ok && mbar_wait_warp(&sm->own[st], own_ph, abort);
-            own_ph ^= 1u;
-        };
-        for (w.start(p, start); w.live() && ok; it_base += w.count, w.next(p)) {
+        w.start(p, start);
+        if (w.live() && !q_tokens) {                            // the first item's Q; a warp of its own fetches the others' ahead
+            copy_q((uint32_t)warp, Plan::kSoftmaxWarps);
+            sync_all();
+            if (tid == 0) mbar_arrive(&sm->q_full);
+        }
+        for (; w.live() && ok; it_base += w.count, w.next(p), ++segment) {
             const uint32_t rows = rows_of(w);
             const bool two = NS == 2 && rows > 128u;            // two tiles of rows
             const uint32_t row0 = w.tile * Plan::kRows + (two ? 128u * st : 0u), item_row = row0 + r;
@@ -145,7 +185,7 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
             const uint32_t token = item_row / p.group;
             const int cached = (int)w.q.n.cached, end = cached + (int)w.q.n.fresh, seen = live ? cached + (int)token + 1 : cached;
             const uint64_t mask = p.tree && live ? p.ancestors[w.q.n.token + token] : 0ull;
-            const int safe = p.tree ? cached : cached + (int)(w.tile * Plan::kRows / p.group) + 1;      // keys before it are seen by every row
+            const int safe = safe_keys(w);
             const uint32_t stride = two ? 1u : NS, begin = two ? 0u : (uint32_t)st;
             float m = -INFINITY, l = 0.0f;
             bool any = false;
@@ -168,61 +208,21 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                 if (lane == 0) mbar_arrive(&sm->s_free[buffer]);
                 const uint32_t bad = sm->bad_keys[it % Plan::kBadRing];      // groups of 16 keys whose page is none
                 if (base + BK > safe || bad) {
-                    // ---- keys that not every row sees
-                    uint32_t sees[BK / 32], odd[BK / 32];
+                    // ---- keys that not every row sees (their values are looked over by the warp that issues the products)
 #pragma unroll
                     for (int i = 0; i < BK / 64; ++i) {
-                        const uint64_t x = paged_sees(p.tree, base + 64 * i, cached, seen, mask) & low_bits(end - base - 64 * i);
-                        sees[2 * i] = (uint32_t)x;
-                        sees[2 * i + 1] = (uint32_t)(x >> 32);
-                    }
+                        uint64_t sees = paged_sees(p.tree, base + 64 * i, cached, seen, mask) & low_bits(end - base - 64 * i);
 #pragma unroll
-                    for (int i = 0; i < BK / 32; ++i) {
-                        const uint32_t b2 = (bad >> (2 * i)) & 3u;
-                        sees[i] &= ~((b2 & 1u ? 0xffffu : 0u) | (b2 & 2u ? 0xffff0000u : 0u));
-                        odd[i] = 0;
-                    }
-                    if (base + BK > safe) {
-                        // A weight of zero times an infinity would reach rows that do not see it, so such values (and whatever lies behind the
-                        // request's end) are taken out of the V tile, and rows that see one of the former are marked. Both streams of an item of two tiles
-                        // read the tile: they clean it together.
-                        uint32_t *found = two ? sm->odd[2][odd_all] : sm->odd[st][odd_own];
-                        const int threads = two ? 256 : 128, at = two ? tid : r;
-                        if (two) odd_all ^= 1u; else odd_own ^= 1u;
-                        if (at < 4) found[at] = 0u;
-                        // (the products of the block before have read theirs, so the tile's barrier is in this block's phase)
-                        if (any) ok = mbar_wait_warp(&sm->o_done[st], done & 1u, abort);
-                        ok = ok && mbar_wait_warp(&sm->v_full[it % kStages], (it / kStages) & 1u, abort);
-                        if (two) sync_all(); else sync_own();
-                        if (ok) {
-                            uint8_t *tile = v_tiles + (it % kStages) * kTileBytes;
-#pragma unroll 4
-                            for (int i = at; i < (int)(kTileBytes / 16); i += threads) {
-                                const int key = (i >> 3) % BK;
-                                if (base + key < cached) continue;
-                                uint4 *x = reinterpret_cast<uint4 *>(tile) + i;
-                                if (base + key >= end) {
-                                    *x = make_uint4(0, 0, 0, 0);
-                                } else {
-                                    const uint4 v = *x;
-                                    const uint32_t a = odd_halves<T>(v.x), b = odd_halves<T>(v.y), c = odd_halves<T>(v.z), d = odd_halves<T>(v.w);
-                                    if (a | b | c | d) {
-                                        atomicOr(&found[key >> 5], 1u << (key & 31));
-                                        *x = make_uint4(without_halves(v.x, a), without_halves(v.y, b), without_halves(v.z, c), without_halves(v.w, d));
-                                    }
-                                }
-                            }
+                        for (int g = 0; g < 4; ++g)
+                            if ((bad >> (4 * i + g)) & 1u) sees &= ~(0xffffull << (16 * g));
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t x = (uint32_t)(sees >> (32 * h));
+                            if (__all_sync(0xffffffffu, x == ~0u)) continue;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) s[64 * i + 32 * h + e] = (x >> e) & 1u ? s[64 * i + 32 * h + e] : -INFINITY;
                         }
-                        fence_proxy_async();
-                        if (two) sync_all(); else sync_own();
-                        if (!ok) break;
-#pragma unroll
-                        for (int i = 0; i < BK / 32; ++i) odd[i] = found[i];
                     }
-#pragma unroll
-                    for (int i = 0; i < BK; ++i) s[i] = (sees[i >> 5] >> (i & 31)) & 1u ? s[i] : -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < BK / 32; ++i) if (odd[i] & sees[i]) l = NAN;
                 }
                 // ---- the block's maximum; O follows it only when it must
                 float t[4] = {s[0], s[1], s[2], s[3]};
@@ -236,24 +236,21 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                 float f = 1.0f;
                 if (m == -INFINITY) m = top;                    // nothing seen so far: O is zero
                 else if (top > m + kSlack) { f = exp2f(m - top); m = top; }
-                if (any) {                                      // the products of the block before: P may be written, O is complete
-                    ok = mbar_wait_warp(&sm->o_done[st], done & 1u, abort);
+                if (__any_sync(0xffffffffu, f != 1.0f)) {
+                    ok = mbar_wait_warp(&sm->o_done[st], done & 1u, abort);      // O is complete
                     if (!ok) break;
                     tc_fence_after();
-                    if (__any_sync(0xffffffffu, f != 1.0f)) {
-                        l *= f;
+                    l *= f;
 #pragma unroll 1
-                        for (int i = 0; i < D; i += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(o_at + i, o);
-                            tmem_ld_wait();
+                    for (int i = 0; i < D; i += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_at + i, o);
+                        tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st16(o_at + i, o);
-                        }
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st16(o_at + i, o);
                     }
                 }
-                any = true;
                 // ---- weights, their sum, and P
                 const float shift = (m == -INFINITY ? 0.0f : m) - kLift;
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -268,21 +265,30 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                         add2(sum[i & 1], x);
                         pk[i] = close2<T>(x.x, x.y);
                     }
+                    if (b == 0 && any) {                        // the products of the block before have read its P
+                        ok = mbar_wait_warp(&sm->o_done[st], done & 1u, abort);
+                        tc_fence_after();
+                    }
                     tmem_st16(p_at + 16 * b, pk);
                 }
+                any = true;
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_st_wait();
+                if (!ok) break;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm->p_full[st]);
             }
             if (!ok) break;
             // ---- the item's end: the last products, then the rows
-            if (any) {
-                ok = mbar_wait_warp(&sm->o_done[st], (done - 1u) & 1u, abort);
-                if (!ok) break;
-                tc_fence_after();
-            }
+            if (any) ok = mbar_wait_warp(&sm->o_done[st], (done - 1u) & 1u, abort);
+            ok = ok && mbar_wait_warp(&sm->looked, segment & 1u, abort);
+            if (!ok) break;
+            tc_fence_after();
+            // a row that sees a value which is not finite
+            if (p.tree ? (mask & sm->odd_mask) != 0 : sm->odd_first < seen - cached) l = NAN;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm->noted);
             float f0 = 1.0f, f1 = 0.0f;                         // factors of the streams' sums
             uint32_t col = 0, cols = D;                         // columns that this thread writes
             const bool share = NS == 2 && !two;
@@ -308,8 +314,18 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
             float *slot = paged_slot(p, blockIdx.x, w.begins, Plan::kRows, D);
             if (!whole && live && col == 0) *reinterpret_cast<float2 *>(slot + 2 * slot_row) = make_float2(m, l);
             const uint32_t o0 = tmem + lanes + Plan::kOCol + (two ? (uint32_t)st * D : 0u);
-            const uint64_t heads = (uint64_t)p.kv_heads * p.group;
-            uint4 *turn = sm->staging[warp];
+            // whole rows go out turned in shared memory, 32 rows x 64 bytes at a time, so that four lanes write a row's 64 bytes instead of one lane
+            // its 16: this lane writes rows 8 e + lane / 4 of the warp's 32
+            uint4 *turn = sm->staging[warp], *to[4];
+            float finite = 0.0f;                                // NaN once a value is not
+            if (whole) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t row = row0 + 32u * (warp & 3) + 8u * e + (lane >> 2), t = row / p.group;
+                    const uint64_t at = ((uint64_t)(w.q.n.token + t) * p.kv_heads + w.head) * p.group + (row - t * p.group);
+                    to[e] = row < w.q.rows ? reinterpret_cast<uint4 *>(p.out + at * D) + (lane & 3) : nullptr;
+                }
+            }
 #pragma unroll 1
             for (uint32_t c = col; c < col + cols; c += 32) {
                 uint32_t a[32];
@@ -328,14 +344,14 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                     }
                 }
                 if (whole) {
-                    // 32 rows x 64 bytes turned in shared memory, so that four lanes write a row's 64 bytes instead of one lane its 16
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         uint32_t o[4];
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
                             const float y0 = __uint_as_float(a[8 * e + 2 * x]) * inv, y1 = __uint_as_float(a[8 * e + 2 * x + 1]) * inv;
-                            bad_out |= live && (!isfinite(y0) || !isfinite(y1));
+                            finite = fmaf(y0, 0.0f, finite);
+                            finite = fmaf(y1, 0.0f, finite);
                             o[x] = close2<T>(y0, y1);
                         }
                         turn[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_uint4(o[0], o[1], o[2], o[3]);
@@ -344,10 +360,7 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int q = 8 * e + (lane >> 2);
-                        const uint32_t row = row0 + 32u * (warp & 3) + q;
-                        const uint4 x = turn[q * 4 + ((lane & 3) ^ ((q >> 1) & 3))];
-                        if (row < w.q.rows)
-                            *reinterpret_cast<uint4 *>(p.out + ((w.q.n.token + row / p.group) * heads + (uint64_t)w.head * p.group + row % p.group) * D + c + 8 * (lane & 3)) = x;
+                        if (to[e]) to[e][c / 8] = turn[q * 4 + ((lane & 3) ^ ((q >> 1) & 3))];
                     }
                     __syncwarp();
                 } else if (live) {
@@ -357,6 +370,7 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                         part[e * Plan::kRows] = make_float4(__uint_as_float(a[4 * e]), __uint_as_float(a[4 * e + 1]), __uint_as_float(a[4 * e + 2]), __uint_as_float(a[4 * e + 3]));
                 }
             }
+            bad_out |= live && finite != finite;
             if (tid == 0 && w.begins && !w.ends)
                 p.share[blockIdx.x] = PagedShare{w.last_cta(start), (int32_t)rows, (int32_t)w.q.n.token, (int32_t)(w.head * p.group),
                                                  (int32_t)(w.tile * Plan::kRows), {0, 0, 0}};
@@ -465,14 +479,19 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
         if (elect_one()) {
             constexpr uint32_t kIdesc = idesc_16bit(!kHalfType, true, D);
             const uint64_t v0 = smem_desc_n_major_sw128(smem_u32(v_tiles), BK * 128);
-            uint32_t it = 0, given[2] = {0, 0};
+            uint32_t it = 0, given[2] = {0, 0}, cleaned = 0;      // cleaned: the phase of each stage's barrier, a bit each
             bool ok = true;
             for (; w.live() && ok; w.next(p)) {
                 const bool two = NS == 2 && rows_of(w) > 128u;
+                const int safe = safe_keys(w);
                 for (uint32_t j = 0; j < w.count && ok; ++j, ++it) {
                     const uint32_t s = it % kStages;
                     const uint64_t vd = v0 + s * (kTileBytes >> 4);
                     ok = mbar_wait(&sm->v_full[s], (it / kStages) & 1u, abort);
+                    if (ok && (int)(w.first + j + 1) * BK > safe) {
+                        ok = mbar_wait(&sm->v_clean[s], (cleaned >> s) & 1u, abort);
+                        cleaned ^= 1u << s;
+                    }
 #pragma unroll
                     for (uint32_t st = 0; st < NS; ++st) {
                         if (!ok || (!two && NS == 2 && (j & 1u) != st)) continue;
@@ -496,28 +515,86 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
             }
         }
     } else if (warp == Plan::kSoftmaxWarps + 3) {
-        // ---------------- Q: rows of an item while the one before is being finished, K-major with the 128-byte swizzle ----------------
-        constexpr int kLanes = D / 8, kAt = 32 / kLanes;         // lanes of a row, rows at a time
-        const uint32_t chunk = (uint32_t)lane % kLanes;
+        // ---------------- what comes once an item: values that are not finite, and the next item's Q ----------------
+        // A weight of zero times an infinity would reach rows that do not see it. So in blocks that not every row sees to the end, values
+        // that are not finite are taken out of the V tile before the products, and noted where they are a fresh token's: rows that see it become
+        // NaN when the item ends. (The softmax warps did this for 8000 cycles a block, two joint waits among them.)
         bool ok = true;
-        for (uint32_t segment = 0; w.live() && ok; w.next(p), ++segment) {
-            if (segment) ok = mbar_wait_warp(&sm->q_free, (segment - 1u) & 1u, abort);
+        uint32_t it = 0, segment = 0;
+        if (q_tokens && w.live() && lane == 0) load_q();
+        while (w.live() && ok) {
+            if (segment) ok = mbar_wait_warp(&sm->noted, (segment - 1u) & 1u, abort);      // the notes on the item before have been read
             if (!ok) break;
-            const uint32_t rows = rows_of(w), tiles = NS == 2 && rows > 128u ? 2u : 1u;
-#pragma unroll 4
-            for (uint32_t row = (uint32_t)lane / kLanes; row < 128u * tiles; row += kAt) {
-                const bool live = row < rows;
-                const uint32_t at = live ? w.tile * Plan::kRows + row : 0u, token = at / p.group;
-                const uint16_t *src = p.q + (uint64_t)(w.q.n.token + token) * p.q_stride + ((uint64_t)w.head * p.group + at % p.group) * D + 8 * chunk;
-                const uint32_t rr = row & 127u;
-                copy16(q_tiles + (row >> 7) * kQBytes + (chunk >> 3) * 16384 + rr * 128 + (((chunk & 7u) ^ (rr & 7u)) << 4), src, live);
-            }
-            copies_done();
-            fence_proxy_async();
+            const int cached = (int)w.q.n.cached, end = cached + (int)w.q.n.fresh, safe = safe_keys(w);
+            if (lane == 0) { sm->odd_mask = 0ull; sm->odd_first = INT32_MAX; }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sm->q_full);
+            for (uint32_t j = 0; j < w.count && ok; ++j) {
+                const uint32_t s = (it + j) % kStages;
+                const int base = (int)(w.first + j) * BK;
+                // (every tile is waited for and let go here too, so that none can be replaced unseen: a barrier's parity only tells a phase from the next)
+                ok = mbar_wait_warp(&sm->v_full[s], ((it + j) / kStages) & 1u, abort);
+                if (!ok) break;
+                if (base + BK <= safe) {
+                    if (lane == 0) mbar_arrive(&sm->v_empty[s]);
+                    continue;
+                }
+                uint4 *tile = reinterpret_cast<uint4 *>(v_tiles + s * kTileBytes);
+                // four keys of 128 bytes at a time, a half of D after the other: zeros behind the request's end; of the fresh tokens' values 0 times
+                // each is summed, which is NaN once one is not finite
+                const int stop = min(BK, max(end - base, 0));
+                for (int h = 0; h < kHalves; ++h) {
+                    uint4 *half = tile + h * BK * 8 + (lane & 7);
+#pragma unroll 4
+                    for (int key = stop + (lane >> 3); key < BK; key += 4) half[key * 8] = make_uint4(0, 0, 0, 0);
+                    for (int key0 = max(safe - base, 0); key0 < stop; key0 += 32) {
+                        typename PairOf<T>::type sum = pair_of<T>(0u);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int key = min(key0 + 4 * e + (lane >> 3), stop - 1);
+                            const uint4 v = half[key * 8];
+                            sum = __hfma2(pair_of<T>(v.x), pair_of<T>(0u), sum);
+                            sum = __hfma2(pair_of<T>(v.y), pair_of<T>(0u), sum);
+                            sum = __hfma2(pair_of<T>(v.z), pair_of<T>(0u), sum);
+                            sum = __hfma2(pair_of<T>(v.w), pair_of<T>(0u), sum);
+                        }
+                        if (!odd_halves<T>(*reinterpret_cast<uint32_t *>(&sum))) continue;
+                        for (int e = 0; e < 8; ++e) {
+                            const int key = key0 + 4 * e + (lane >> 3), fresh = base + key - cached;
+                            if (key >= stop) break;
+                            const uint4 v = half[key * 8];
+                            const uint4 o = make_uint4(odd_halves<T>(v.x), odd_halves<T>(v.y), odd_halves<T>(v.z), odd_halves<T>(v.w));
+                            if (!(o.x | o.y | o.z | o.w)) continue;
+                            half[key * 8] = make_uint4(without_halves(v.x, o.x), without_halves(v.y, o.y), without_halves(v.z, o.z), without_halves(v.w, o.w));
+                            if (fresh < YVEX_B200_TREE_NODES) atomicOr(&sm->odd_mask, 1ull << fresh);
+                            atomicMin(&sm->odd_first, fresh);
+                        }
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(&sm->v_clean[s]); mbar_arrive(&sm->v_empty[s]); }
+            }
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(&sm->looked);
+            it += w.count;
+            w.next(p);
+            if (!ok || !w.live()) break;
+            ok = mbar_wait_warp(&sm->q_free, segment & 1u, abort);
+            if (!ok) break;
+            if (q_tokens) {
+                if (lane == 0) load_q();
+            } else {
+                copy_q(0, 1);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm->q_full);
+            }
+            ++segment;
         }
-        copies_done();
+        if (!ok && lane == 0 && q_tokens) {                     // Q in flight must land before the CTA ends
+            volatile int none = 0;
+            mbar_wait(&sm->q_full, segment & 1u, &none, 1000000ull);
+        }
+        __syncwarp();
     }
     }
     tc_fence_before();
@@ -549,6 +626,17 @@ static int pages_map(CUtensorMap *map, const uint16_t *base, const PagedParams &
     return r == CUDA_SUCCESS ? OK : ERR_BACKEND;
 }
 
+static int rows_map(CUtensorMap *map, const PagedParams &p, unsigned qtype, uint64_t head_dim) {
+    auto fn = tiles_encode();
+    if (!fn) return ERR_BACKEND;
+    cuuint64_t dims[3] = {head_dim, (cuuint64_t)p.kv_heads * p.group, p.tokens}, strides[2] = {head_dim * 2, p.q_stride * 2};
+    cuuint32_t box[3] = {64, p.group, 128 / p.group}, estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, qtype == Q_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<uint16_t *>(p.q), dims,
+                          strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? OK : ERR_BACKEND;
+}
+
 template <class T, int D> static int launch_tiles(const PagedParams &p, unsigned qtype, unsigned ctas, cudaStream_t s) {
     using Plan = TilePlan<D>;
     static SmemOptIn optin;
@@ -559,8 +647,10 @@ template <class T, int D> static int launch_tiles(const PagedParams &p, unsigned
     int box = 16;                                               // a box stays within a page
     while (box < Plan::kKeys && p.page_size % (2u * box) == 0) box *= 2;
     TileMaps maps;
+    const int q_tokens = p.group <= 128 && 128 % p.group == 0 ? (int)(128 / p.group) : 0;
+    if (q_tokens && rows_map(&maps.q, p, qtype, D) != OK) return ERR_BACKEND;
     if (pages_map(&maps.k, p.k, p, qtype, D, box) != OK || pages_map(&maps.v, p.v, p, qtype, D, box) != OK) return ERR_BACKEND;
-    if (launch_pdl(paged_tiles_kernel<T, D>, dim3(ctas), dim3(Plan::kThreads), smem, s, maps, p, box) != cudaSuccess) return ERR_BACKEND;
+    if (launch_pdl(paged_tiles_kernel<T, D>, dim3(ctas), dim3(Plan::kThreads), smem, s, maps, p, box, q_tokens) != cudaSuccess) return ERR_BACKEND;
     return OK;
 }
 

@@ -65,7 +65,9 @@ template <int MROWS, int BK> struct PagedRequest {
 
 // Where a CTA's share begins, found by all its threads (NT of them). COST: what beginning and ending an item costs, in blocks; they
 // stand before the item's first block when the shares are cut.
-struct PagedStart { uint64_t total, from, left; uint32_t request, head, tile, skip, ctas; };
+struct PagedStart { uint64_t total, each, from, left; uint32_t more, request, head, tile, skip, ctas; };
+// (a 64-bit division takes hundreds of cycles)
+__device__ __forceinline__ uint64_t divided(uint64_t a, uint64_t b) { return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b; }
 template <int NT> struct PagedScratch {
     uint64_t warps[NT / 32], sum, skip;
     uint32_t request, head, tile, first;
@@ -132,10 +134,12 @@ __device__ PagedStart paged_start(const PagedParams &p, PagedScratch<NT> *sc) {
     uint64_t prefix = scan(v);
     st.total = sc->sum * p.kv_heads;
     st.ctas = (uint32_t)min((uint64_t)gridDim.x, st.total);     // every CTA that has a share has a unit at least
-    const uint64_t u0 = blockIdx.x < st.ctas ? st.total * blockIdx.x / st.ctas : st.total;
-    const uint64_t u1 = blockIdx.x < st.ctas ? st.total * (blockIdx.x + 1ull) / st.ctas : st.total;
+    // `more` CTAs have one unit more than `each`
+    st.each = st.ctas ? divided(st.total, st.ctas) : 0;
+    st.more = (uint32_t)(st.total - st.each * st.ctas);
+    const uint64_t u0 = blockIdx.x < st.ctas ? st.each * blockIdx.x + min(blockIdx.x, st.more) : st.total;
     st.from = u0;
-    st.left = u1 - u0;
+    st.left = blockIdx.x < st.ctas ? st.each + (blockIdx.x < st.more ? 1 : 0) : 0;
     uint64_t base = 0;
     for (uint64_t chunk = 0; chunk < p.requests && st.left; chunk += NT) {
         if (!single) {
@@ -145,7 +149,7 @@ __device__ PagedStart paged_start(const PagedParams &p, PagedScratch<NT> *sc) {
         }
         const uint64_t begin = (base + prefix - v) * p.kv_heads;
         if (v && u0 >= begin && u0 < begin + v * p.kv_heads) {
-            const uint64_t skip = u0 - begin, head = skip / v;
+            const uint64_t skip = u0 - begin, head = divided(skip, v);
             sc->request = (uint32_t)(chunk + tid);
             sc->head = (uint32_t)head;
             sc->skip = skip - head * v;
@@ -224,7 +228,10 @@ template <int MROWS, int BK, int COST> struct PagedWalk {
         cut(p, 0);
     }
     // The CTA that holds the item's last block; of a segment that does not end its item.
-    __device__ __forceinline__ int32_t last_cta(const PagedStart &s) const { return (int32_t)(((at + rest) * s.ctas - 1) / s.total); }
+    __device__ __forceinline__ int32_t last_cta(const PagedStart &s) const {
+        const uint64_t u = at + rest - 1, larger = s.more * (s.each + 1);
+        return (int32_t)(u < larger ? divided(u, s.each + 1) : s.more + divided(u - larger, s.each));
+    }
 };
 
 // A slot of the workspace: (maximum, sum) of every row, then the accumulators in groups of four columns, [head_dim / 4][rows][4], so that
