@@ -611,6 +611,17 @@ def test_logits_long_history_and_no_history(L):
     assert torch.equal(L.logits_edit(bare, plain, x, st), x) and st.read() == 0
 
 
+@pytest.mark.parametrize("vocabulary,biases", [(700, 500), (40000, 3000)])
+def test_logits_many_biases(L, vocabulary, biases):
+    """More entries than a CTA lists, words among them several times: the last entry counts."""
+    import torch
+    policy, drafts, x, mask, want, request = edit_case(L, vocabulary, [2, 1], False, "float32", biases=biases, seed=biases)
+    st = L.Status()
+    out = L.logits_edit(policy, drafts, x, st, grammar=mask)
+    assert st.read() == 0
+    check_edit(out, want, request, out)
+
+
 def test_logits_infinities_and_nan(L):
     """Infinities pass; NaN in a place that the grammar forbids is gone, in an allowed one it stays and is reported."""
     import torch

@@ -26,7 +26,10 @@ struct PagedParams {
     struct PagedShare *share;                    // [CTAs]
 };
 
-constexpr int kTilesCost = 2;                    // of the tiles kernel, in its blocks of 128 keys (64 with 256 dims)
+// What an item costs the tiles kernel besides its blocks of 128 keys (64 with 256 dims), in blocks: the first S waits for Q, the last PV is
+// waited for, the sums are read and written, and the code of all that is fetched anew. (16 trees at 100 to 32768 keys: 2 blocks 283 us,
+// 4 287, 6 253; chunks of two prompts 570, 560, 550.)
+constexpr int kTilesCost = 6;
 
 // An item that a CTA began: CTAs c .. last hold its parts. rows 0: none.
 struct PagedShare { int32_t last, rows, token, head, first_row, pad[3]; };
