@@ -622,6 +622,28 @@ def test_logits_many_biases(L, vocabulary, biases):
     check_edit(out, want, request, out)
 
 
+def test_logits_more_words_than_a_table_holds(L):
+    """A history with tens of thousands of different words, over one row and over several, with paths and biases among them."""
+    import torch
+    for fresh, tree in (([1], False), ([5, 3], False), ([20], True)):
+        policy, drafts, x, mask, want, request = edit_case(L, 60000, fresh, tree, "float32", history=10, biases=2000, seed=len(fresh))
+        words = torch.randperm(60000, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(torch.int32)
+        R = len(fresh)
+        p2 = L.logits_policy_of(60000, words, ints([0] + [60000] * R), ints([40000] * R), *policy._keep[3:])
+        st = L.Status()
+        out = L.logits_edit(p2, drafts, x, st, grammar=mask)
+        assert st.read() == 0
+        k = policy._keep
+        hist = [words.tolist()] + [[]] * (R - 1)
+        off, bo = drafts._keep[2].tolist(), k[8].tolist()
+        bias = [list(zip(k[6].tolist()[bo[r]:bo[r + 1]], k[7].tolist()[bo[r]:bo[r + 1]])) for r in range(R)]
+        drafted, masks = drafts._keep[0].tolist(), drafts._keep[3].tolist() if tree else None
+        paths = [[] if r < 0 else [drafted[off[r] + j] for j in range(fresh[r]) if (masks[t] >> j & 1 if tree else j <= t - off[r])] for t, r in enumerate(request)]
+        f64 = [k[i].double().cpu().numpy() for i in (3, 4, 5)]
+        want = O.logits(x.double().cpu().numpy(), request, hist, [40000] * R, *f64, bias, paths, mask.cpu().numpy(), 60000)
+        check_edit(out, want, request, out)
+
+
 def test_logits_infinities_and_nan(L):
     """Infinities pass; NaN in a place that the grammar forbids is gone, in an allowed one it stays and is reported."""
     import torch
