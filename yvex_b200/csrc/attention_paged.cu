@@ -239,8 +239,9 @@ __global__ void __launch_bounds__(kRowsThreads, R == 8 && D <= 128 ? 3 : 2) page
 }
 
 // Joins the parts of the item that CTA blockIdx.x of the kernel before began and did not end: a CTA takes eight rows, a thread four
-// columns of one of them (a warp's 8 rows x 16 columns are whole lines of every part, and whole sectors of the output). The parts are
-// walked twice, for their maximum and then for their sums; all loads of a walk are independent.
+// columns of one of them (a warp's 8 rows x 16 columns are whole lines of every part, and whole sectors of the output). One walk over the
+// parts with a running maximum, four loads ahead: with a walk for the maximum first, or more loads ahead, it took 1 to 3 us more at 20 parts,
+// since the code is fetched anew by every call.
 constexpr int kJoinRows = 8;
 template <class T, int D>
 __global__ void __launch_bounds__(2 * D) paged_join_kernel(const PagedParams p, int slot_rows) {
@@ -251,19 +252,20 @@ __global__ void __launch_bounds__(2 * D) paged_join_kernel(const PagedParams p, 
     if (row >= sh.rows) return;
     const uint64_t pitch = paged_slot_floats((uint32_t)slot_rows, D);
     const int parts = sh.last - (int)blockIdx.x + 1;
-    auto slot = [&](int i) { return p.partial + (2ull * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * pitch; };
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) top = fmaxf(top, slot(i)[2 * row]);
-    float sum = 0.0f;
+    const float *slot = p.partial + (2ull * blockIdx.x + 1) * pitch;      // the first part; the others are every second slot from the next one on
+    const uint32_t ml_at = 2u * row, acc_at = 2u * slot_rows + 4u * (group * slot_rows + row);
+    float top = -INFINITY, sum = 0.0f;
     float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
     for (int i = 0; i < parts; ++i) {
-        const float2 ml = *reinterpret_cast<const float2 *>(slot(i) + 2 * row);
-        const float4 y = *reinterpret_cast<const float4 *>(slot(i) + 2 * slot_rows + (group * slot_rows + row) * 4);
-        const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
-        sum += ml.x == -INFINITY ? ml.y : ml.y * f;
-        a.x += y.x * f; a.y += y.y * f; a.z += y.z * f; a.w += y.w * f;
+        const float2 ml = *reinterpret_cast<const float2 *>(slot + ml_at);
+        const float4 y = *reinterpret_cast<const float4 *>(slot + acc_at);
+        slot += i == 0 ? pitch : 2 * pitch;
+        const float most = fmaxf(top, ml.x), shift = most == -INFINITY ? 0.0f : most;
+        const float c = exp2f(top - shift), f = exp2f(ml.x - shift);      // (a part that saw nothing: 0, and its sum is 0, or NaN where it marks the row)
+        top = most;
+        sum = sum * c + (ml.x == -INFINITY ? ml.y : ml.y * f);
+        a.x = a.x * c + y.x * f; a.y = a.y * c + y.y * f; a.z = a.z * c + y.z * f; a.w = a.w * c + y.w * f;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
