@@ -136,8 +136,8 @@ def test_python_front_end_refuses_what_it_can_see(L, monkeypatch):
     import torch
     from types import SimpleNamespace as N
     monkeypatch.setattr(L, "_torch", lambda: torch)
-    monkeypatch.setattr(L, "_here", lambda t: t.device.type == "cpu")
-    monkeypatch.setattr(L, "_stream", lambda: None)
+    monkeypatch.setattr(L, "_device", lambda: -1)                # where a host tensor says it is
+    monkeypatch.setattr(L, "_on", lambda dev: None)
     called = []
     monkeypatch.setattr(L, "lib", N(yvex_b200_kv_append=lambda *a: called.append(a) or 0, yvex_b200_kv_plan=lambda *a: called.append(a) or 0,
                                     yvex_b200_attention_paged=lambda *a: called.append(a) or 0, yvex_b200_logits_edit=lambda *a: called.append(a) or 0))
@@ -146,15 +146,13 @@ def test_python_front_end_refuses_what_it_can_see(L, monkeypatch):
     for bad in ((k, k.half()), (k, k[:3]), (k[0], k[0]), (k.transpose(0, 1), k.transpose(0, 1)), (k.float(), k.double())):
         with pytest.raises(L.YvexError):
             L.kv_cache_of(*bad)
-    with pytest.raises(L.YvexError):
-        L.kv_cache_of(k.to("meta"), k.to("meta"))
     c = L.kv_cache_of(k, k)
     assert (c.qtype, c.pages, c.kv_heads, c.page_size, c.head_dim) == (30, 4, 2, 16, 64)
     good = dict(cached=i32(3), fresh=i32(3), block_table=i32(3, 5), tokens=7, longest_fresh=3, longest=50)
     s = L.kv_step_of(**good)
     assert (s.requests, s.tokens, s.table_width, s.tree, s.parents, s.ancestors) == (3, 7, 5, 0, None, None)
     for n, x in (("cached", torch.zeros(3)), ("fresh", i32(2)), ("block_table", i32(2, 5)), ("block_table", i32(5, 3).T), ("parents", i32(6)), ("offsets", i32(3)),
-                 ("slots", i32(7)), ("positions", i32(6)), ("cached", i32(6)[::2]), ("fresh", i32(3).to("meta"))):
+                 ("slots", i32(7)), ("positions", i32(6)), ("cached", i32(6)[::2])):
         with pytest.raises(L.YvexError):
             L.kv_step_of(**dict(good, **{n: x}))
     rows, slots = torch.zeros((7, 2, 2, 64)), torch.zeros(7, dtype=torch.int64)
@@ -186,6 +184,13 @@ def test_python_front_end_refuses_what_it_can_see(L, monkeypatch):
         L.logits_policy_of(100)
     with pytest.raises(L.YvexError):
         L.logits_drafts_of(i32(3), i32(4))
+    # tensors of another device than the current one
+    monkeypatch.setattr(L, "_device", lambda: 0)
+    for call in (lambda: L.kv_cache_of(k, k), lambda: L.kv_step_of(**good), lambda: L.kv_plan(c, s, i32(3), st, i32(1)), lambda: L.kv_append(c, slots, rows[:, 0], rows[:, 1], st),
+                 lambda: L.attention_paged(c, s, q, 0.1, st, workspace=ws), lambda: L.logits_edit(p, d, x, st), lambda: L.logits_policy_of(9, i32(1), i32(2)),
+                 lambda: L.logits_drafts_of(i32(3), i32(3))):
+        with pytest.raises(L.YvexError):
+            call()
     assert not called
 
 

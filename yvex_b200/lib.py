@@ -537,22 +537,34 @@ def _need(ok, where):
         raise YvexError(INVALID_ARG, where)
 
 
-def _here(t):
-    """The tensor lies on the current device, whose current stream the call goes to."""
-    return t.is_cuda and t.get_device() == _torch().cuda.current_device()
+def _device():
+    """Index of the current device, whose current stream a call goes to (the private call where torch has it: 0.4 us less)."""
+    get = getattr(_torch()._C, "_cuda_getDevice", None)
+    return get() if get else _torch().cuda.current_device()
 
 
-def _array(t, dtype, numel, where):
-    """A packed device array of the given type with at least `numel` elements (None: whatever it has), or None."""
-    _need(t is None or (t.dtype == dtype and t.is_contiguous() and _here(t) and (numel is None or t.numel() >= numel)), where)
-    return _p(t)
+def _on(dev):
+    """Raw handle of the device's current stream."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(dev) if raw else torch.cuda.current_stream(dev).cuda_stream
+
+
+def _array(t, dtype, numel, where, dev):
+    """Address of a packed array of the given type on device `dev` with at least `numel` elements (None: whatever it has); None for None."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.get_device() != dev or not t.is_contiguous() or (numel is not None and t.numel() < numel):
+        raise YvexError(INVALID_ARG, where)
+    return t.data_ptr()
 
 
 def _row_stride(t, where):
     """Elements between the rows of [rows, heads, dim] values whose rows are packed."""
     rows, heads, dim = t.shape
-    _need((t.stride(2) == 1 or dim == 1) and (t.stride(1) == dim or heads == 1), where)
-    return t.stride(0) if rows > 1 else heads * dim
+    between, inner, one = t.stride()
+    _need(one == 1 and (inner == dim or heads == 1), where)
+    return between if rows > 1 else heads * dim
 
 
 def kv_geometry_of(pages, page_size):
@@ -561,11 +573,13 @@ def kv_geometry_of(pages, page_size):
 
 
 def kv_cache_of(k, v):
-    """Description of a paged cache: k, v [pages, kv_heads, page_size, head_dim] of f16 or bf16, packed."""
-    _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous() and _here(k) and _here(v), "kv_cache_of")
+    """Description of a paged cache: k, v [pages, kv_heads, page_size, head_dim] of f16 or bf16, packed, on the current device."""
+    dev = _device()
+    _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous() and k.get_device() == v.get_device() == dev,
+          "kv_cache_of")
     pages, heads, page_size, dim = k.shape
     c = KvCache(_qtype_of(k, "kv_cache_of"), pages, page_size, heads, dim, _p(k), _p(v))
-    c._keep, c.dtype = (k, v), k.dtype
+    c._keep, c.dtype, c.row = (k, v), k.dtype, (heads, dim)
     return c
 
 
@@ -576,38 +590,40 @@ def kv_step_of(cached, fresh, block_table, tokens, longest_fresh, longest, paren
     ancestors int64 [tokens] for trees) are made here unless given; they are the step's *_tensor attributes."""
     torch = _torch()
     tree = bool(tree if tree is not None else parents is not None)
-    requests, dev, i32, i64, w = cached.numel(), cached.device, torch.int32, torch.int64, "kv_step_of"
+    requests, where, i32, i64, w = cached.numel(), cached.device, torch.int32, torch.int64, "kv_step_of"
     _need(block_table.dim() == 2 and block_table.shape[0] == requests, w)
-    new = lambda t, n, dtype: torch.empty(n, dtype=dtype, device=dev) if t is None else t  # noqa: E731
+    new = lambda t, n, dtype: torch.empty(n, dtype=dtype, device=where) if t is None else t  # noqa: E731
     offsets, slots = new(offsets, requests + 1, i32), new(slots, tokens, i64)
     positions, row_request = new(positions, tokens, i32), new(row_request, tokens, i32)
     ancestors = new(ancestors, tokens, i64) if tree else None
-    s = KvStep(requests, tokens, block_table.shape[1], longest_fresh, longest, int(tree), _array(cached, i32, requests, w), _array(fresh, i32, requests, w),
-               _array(parents, i32, tokens, w), _array(block_table, i32, None, w), _array(offsets, i32, requests + 1, w), _array(slots, i64, tokens, w),
-               _array(positions, i32, tokens, w), _array(row_request, i32, tokens, w), _array(ancestors, i64, tokens, w))
-    s._keep = (cached, fresh, parents, block_table)
+    dev = _device()
+    at = lambda t, dtype, n: _array(t, dtype, n, w, dev)  # noqa: E731
+    s = KvStep(requests, tokens, block_table.shape[1], longest_fresh, longest, int(tree), at(cached, i32, requests), at(fresh, i32, requests),
+               at(parents, i32, tokens), at(block_table, i32, None), at(offsets, i32, requests + 1), at(slots, i64, tokens),
+               at(positions, i32, tokens), at(row_request, i32, tokens), at(ancestors, i64, tokens))
+    s._keep, s.rows = (cached, fresh, parents, block_table), tokens
     s.offsets_tensor, s.slots_tensor, s.positions_tensor, s.row_request_tensor, s.ancestors_tensor = offsets, slots, positions, row_request, ancestors
     return s
 
 
 def kv_plan(cache, step, free_pages, status, pages_used=None):
     """Plans the step on the device (see yvex_b200_kv_plan); free_pages int32 -> pages_used [1] int32, how many of them it took."""
-    torch = _torch()
+    torch, dev = _torch(), _device()
     if pages_used is None:
         pages_used = torch.empty(1, dtype=torch.int32, device=free_pages.device)
-    _check(lib.yvex_b200_kv_plan(cache, step, _array(free_pages, torch.int32, None, "kv_plan"), free_pages.numel(),
-                                 _array(pages_used, torch.int32, 1, "kv_plan"), _p(status.word), _stream()), "kv_plan")
+    _check(lib.yvex_b200_kv_plan(cache, step, _array(free_pages, torch.int32, None, "kv_plan", dev), free_pages.numel(),
+                                 _array(pages_used, torch.int32, 1, "kv_plan", dev), status.word.data_ptr(), _on(dev)), "kv_plan")
     return pages_used
 
 
 def kv_append(cache, slots, k, v, status):
     """Stores rows k, v [tokens, kv_heads, head_dim] (f32, f16 or bf16; rows may be strided views, as of a fused projection) at
     slots [tokens] int64; negative slots are skipped."""
-    torch, w = _torch(), "kv_append"
-    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
-    _need(k.shape == shape and v.shape == shape and k.dtype == v.dtype and _here(k) and _here(v), w)
-    _check(lib.yvex_b200_kv_append(cache, _array(slots, torch.int64, None, w), slots.numel(), _qtype_of(k, w), _p(k), _row_stride(k, w), _p(v),
-                                   _row_stride(v, w), _p(status.word), _stream()), w)
+    torch, dev, w = _torch(), _device(), "kv_append"
+    tokens, shape = slots.numel(), k.shape
+    _need(shape == v.shape and len(shape) == 3 and shape[0] == tokens and shape[1:] == cache.row and k.dtype == v.dtype and k.get_device() == v.get_device() == dev, w)
+    _check(lib.yvex_b200_kv_append(cache, _array(slots, torch.int64, None, w, dev), tokens, _qtype_of(k, w), k.data_ptr(), _row_stride(k, w), v.data_ptr(),
+                                   _row_stride(v, w), status.word.data_ptr(), _on(dev)), w)
 
 
 def attention_paged_workspace(cache, step, q_heads):
@@ -620,58 +636,68 @@ def attention_paged_workspace(cache, step, q_heads):
 
 def attention_paged(cache, step, q, scale, status, workspace=None, out=None):
     """q [tokens, q_heads, head_dim] in the cache's type (rows may be strided) -> out [tokens, q_heads, head_dim] in the same type."""
-    torch, w = _torch(), "attention_paged"
-    _need(q.dim() == 3 and q.shape[0] == step.tokens and q.shape[2] == cache.head_dim and q.dtype == cache.dtype and _here(q), w)
-    heads = q.shape[1]
+    torch, dev, w = _torch(), _device(), "attention_paged"
+    shape, dtype = q.shape, q.dtype
+    _need(len(shape) == 3 and shape[0] == step.rows and shape[2] == cache.row[1] and dtype == cache.dtype and q.get_device() == dev, w)
+    heads = shape[1]
     if workspace is None:
         workspace = attention_paged_workspace(cache, step, heads)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _check(lib.yvex_b200_attention_paged(cache, step, _p(q), _row_stride(q, w), heads, scale, _array(out, q.dtype, q.numel(), w),
-                                         _array(workspace, torch.uint8, None, w), workspace.numel(), _p(status.word), _stream()), w)
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    _check(lib.yvex_b200_attention_paged(cache, step, q.data_ptr(), _row_stride(q, w), heads, scale, _array(out, dtype, q.numel(), w, dev),
+                                         _array(workspace, torch.uint8, None, w, dev), workspace.numel(), status.word.data_ptr(), _on(dev)), w)
     return out
 
 
 def logits_policy_of(vocabulary, history=None, history_offsets=None, prompt_lengths=None, repetition=None, presence=None, frequency=None,
                      bias_tokens=None, bias_values=None, bias_offsets=None, requests=None):
     """What the requests' logits are edited by: ids int32 packed by offsets [requests + 1] int32, penalties [requests] f32."""
-    torch, w = _torch(), "logits_policy_of"
+    torch, dev, w = _torch(), _device(), "logits_policy_of"
     i32, f32 = torch.int32, torch.float32
     if requests is None:
-        known = [t.numel() - 1 for t in (history_offsets, bias_offsets) if t is not None] +                 [t.numel() for t in (prompt_lengths, repetition, presence, frequency) if t is not None]
+        known = [t.numel() - 1 for t in (history_offsets, bias_offsets) if t is not None] + \
+                [t.numel() for t in (prompt_lengths, repetition, presence, frequency) if t is not None]
         _need(known, w)
         requests = known[0]
     count = lambda t: 0 if t is None else t.numel()  # noqa: E731
-    p = LogitsPolicy(vocabulary, requests, count(history), count(bias_tokens), _array(history, i32, None, w), _array(history_offsets, i32, requests + 1, w),
-                     _array(prompt_lengths, i32, requests, w), _array(repetition, f32, requests, w), _array(presence, f32, requests, w),
-                     _array(frequency, f32, requests, w), _array(bias_tokens, i32, None, w),
-                     _array(bias_values, f32, count(bias_tokens), w), _array(bias_offsets, i32, requests + 1, w))
+    at = lambda t, dtype, n: _array(t, dtype, n, w, dev)  # noqa: E731
+    p = LogitsPolicy(vocabulary, requests, count(history), count(bias_tokens), at(history, i32, None), at(history_offsets, i32, requests + 1),
+                     at(prompt_lengths, i32, requests), at(repetition, f32, requests), at(presence, f32, requests), at(frequency, f32, requests),
+                     at(bias_tokens, i32, None), at(bias_values, f32, count(bias_tokens)), at(bias_offsets, i32, requests + 1))
     p._keep = (history, history_offsets, prompt_lengths, repetition, presence, frequency, bias_tokens, bias_values, bias_offsets)
     return p
 
 
 def logits_drafts_of(drafted=None, row_request=None, offsets=None, ancestors=None, tree=False, rows=None):
     """Which request each row of logits belongs to, and the words drafted for the rows (arrays as kv_plan writes them)."""
-    torch, w = _torch(), "logits_drafts_of"
+    torch, dev, w = _torch(), _device(), "logits_drafts_of"
     if rows is None:
         _need(row_request is not None, w)
         rows = row_request.numel()
-    d = LogitsDrafts(rows, int(tree), _array(drafted, torch.int32, rows, w), _array(row_request, torch.int32, rows, w),
-                     _array(offsets, torch.int32, None, w), _array(ancestors, torch.int64, rows, w))
+    d = LogitsDrafts(rows, int(tree), _array(drafted, torch.int32, rows, w, dev), _array(row_request, torch.int32, rows, w, dev),
+                     _array(offsets, torch.int32, None, w, dev), _array(ancestors, torch.int64, rows, w, dev))
     d._keep, d.requests = (drafted, row_request, offsets, ancestors), None if offsets is None else offsets.numel() - 1
     return d
 
 
 def logits_edit(policy, drafts, logits, status, grammar=None, out=None):
     """logits [rows, vocabulary] f32, f16 or bf16 -> the edited rows (out may be logits itself); grammar [rows, words] int32 bit masks."""
-    torch, w = _torch(), "logits_edit"
-    _need(logits.dim() == 2 and logits.shape[0] >= drafts.rows and logits.shape[1] == policy.vocabulary and logits.stride(1) == 1 and _here(logits), w)
+    torch, dev, w = _torch(), _device(), "logits_edit"
+    shape, rows = logits.shape, drafts.rows
+    _need(len(shape) == 2 and shape[0] >= rows and shape[1] == policy.vocabulary and (shape[1] == 1 or logits.stride(1) == 1) and logits.get_device() == dev, w)
     _need(drafts.requests is None or drafts.requests >= policy.requests, w)
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _need(out.shape == logits.shape and out.dtype == logits.dtype and out.stride(1) == 1 and _here(out), w)
+        out = torch.empty(shape, dtype=logits.dtype, device=logits.device)
+    _need(out.shape == shape and out.dtype == logits.dtype and (shape[1] == 1 or out.stride(1) == 1) and out.get_device() == dev, w)
+    address, words = None, 0
     if grammar is not None:
-        _need(grammar.dim() == 2 and grammar.shape[0] >= drafts.rows and grammar.dtype == torch.int32 and grammar.stride(1) == 1 and _here(grammar), w)
-    _check(lib.yvex_b200_logits_edit(policy, drafts, _qtype_of(logits, w), _p(logits), logits.stride(0), _p(grammar),
-                                     grammar.stride(0) if grammar is not None else 0, _p(out), out.stride(0), _p(status.word), _stream()), w)
+        _need(grammar.dim() == 2 and grammar.shape[0] >= rows and grammar.dtype == torch.int32 and grammar.stride(1) == 1 and grammar.get_device() == dev, w)
+        address, words = grammar.data_ptr(), _pitch(grammar)
+    _check(lib.yvex_b200_logits_edit(policy, drafts, _qtype_of(logits, w), logits.data_ptr(), _pitch(logits), address, words, out.data_ptr(), _pitch(out),
+                                     status.word.data_ptr(), _on(dev)), w)
     return out
+
+
+def _pitch(t):
+    """Elements between the rows of a matrix (its width where it has but one)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
