@@ -443,7 +443,7 @@ int yvex_b200_attention_sink(const float *query, const float *rows, const float 
  * in the reference, whose attention op reads one contiguous session (src/backend/cpu.c:319-411).
  *
  * The cache: k and v are [pages][kv_heads][page_size][head_dim] of F16 (qtype 1) or BF16 (30), 16-byte aligned;
- * page_size is a multiple of 16, head_dim 64, 128 or 256. A cache of whole sessions [sessions][kv_heads][context][head_dim],
+ * page_size is a multiple of 16, head_dim 64, 128 or 256, pages * kv_heads * page_size below 2^31. A cache of whole sessions [sessions][kv_heads][context][head_dim],
  * as yvex_b200_attention_gqa_decode reads it, is the case of one page per session.
  *
  * The step: request r has cached[r] tokens in its pages already and brings fresh[r] more (one, a drafted chain or
@@ -451,7 +451,7 @@ int yvex_b200_attention_sink(const float *query, const float *rows, const float 
  * of all requests are packed rows: those of r are offsets[r] .. offsets[r + 1] - 1. `tokens` is the number of rows the
  * arrays have room for; rows from offsets[requests] on are padding (a captured graph's batch may be larger than the
  * step). longest_fresh and longest bound fresh[r] and cached[r] + fresh[r]; they choose and size launches, the
- * lengths themselves stay on the device. tree: parents[row] is the index of the row's parent among its request's
+ * lengths themselves stay on the device (longest at most 2^30). tree: parents[row] is the index of the row's parent among its request's
  * fresh tokens, below the row's own, or -1 for a child of the last cached token; a tree has at most
  * YVEX_B200_TREE_NODES nodes and ancestors[row] has the bits of the nodes that the row sees, its own among them.
  * Without tree the fresh tokens are a chain: each sees those before it and itself. All lengths, ids and tables are int32

@@ -49,7 +49,7 @@ def edit(L, p=None, d=None, qtype=0, x=P, xs=1000, g=P, gs=32, out=P, os_=1000, 
 
 
 SIZES = [("requests", 0, INVALID), ("tokens", 0, INVALID), ("table_width", 0, INVALID), ("longest_fresh", 0, INVALID), ("longest", 0, INVALID),
-         ("longest_fresh", 81, BOUNDS), ("requests", 1 << 31, BOUNDS), ("tokens", 1 << 31, BOUNDS), ("longest", 1 << 32, BOUNDS), ("table_width", 1 << 32, BOUNDS)]
+         ("longest_fresh", 81, BOUNDS), ("requests", 1 << 31, BOUNDS), ("tokens", 1 << 31, BOUNDS), ("longest", (1 << 30) + 1, BOUNDS), ("table_width", 1 << 32, BOUNDS)]
 
 
 @pytest.mark.parametrize("name,value,code", SIZES)
@@ -110,6 +110,8 @@ def test_attention_refuses_before_launch(L):
     for scale in (0.0, -1.0, float("nan"), float("inf")):
         assert attend(L, scale=scale) == INVALID
     assert attend(L, heads=7) == INVALID and attend(L, heads=0) == INVALID and attend(L, heads=1 << 20, stride=1 << 30) == BOUNDS
+    for pages, heads, size in ((1 << 20, 2, 1024), (1 << 30, 1024, 1 << 24), ((1 << 31) - 1, 2, 16)):      # rows that a 32-bit coordinate cannot name
+        assert attend(L, c=cache(L, pages=pages, kv_heads=heads, page_size=size), heads=heads, stride=1 << 20) == BOUNDS
     assert attend(L, stride=1023) == BOUNDS and attend(L, stride=1028) == INVALID and attend(L, q=P + 8) == INVALID and attend(L, out=P + 2) == INVALID
     assert L.lib.yvex_b200_launch_count() == before
 

@@ -6,6 +6,8 @@
 // of PV whatever keys a lane holds), so nothing is staged or transposed. 16 keys never straddle a page, and the page
 // of a warp's next block is looked up while this one is computed. The weights are rounded once to the cache's type for the second product,
 // which adds less to the output's error than its own rounding (an output of f32 would not allow that); their sum stays f32 and unrounded.
+// 64 sessions of 100 to 32768 keys (3.46 GB): 558 us, 6.2 TB/s, 94 % of the copy bandwidth; equal shares of blocks instead of a fixed number of
+// slices per session are what holds that for ragged lengths. One session of 1500 keys: 12 us for the two kernels, all latency.
 #include <cuda_bf16.h>
 
 #include <initializer_list>
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(2 * D) paged_join_kernel(const PagedParams p, 
 }
 
 // Which kernel, for how many rows a slot holds, on how many CTAs. Up to 16 rows fit the MMA of the rows kernel (8 with 256 dims, where
-// sixteen rows of Q and O would not fit the registers).
+// sixteen rows of Q and O would not fit the registers); beyond that its operands would be read again for every 16 rows, while a tile holds 128.
 struct PagedShape { bool tiles; uint32_t rows; unsigned ctas; };
 static PagedShape paged_shape(const yvex_b200_kv_cache *c, const yvex_b200_kv_step *t, uint64_t q_heads) {
     const uint64_t group = q_heads / c->kv_heads, rows = t->longest_fresh * group, D = c->head_dim;
@@ -322,7 +324,7 @@ static int paged_refusal(const yvex_b200_kv_cache *c, const yvex_b200_kv_step *t
     if (rc == OK) rc = check_step(t);
     if (rc != OK) return rc;
     if (!q_heads || q_heads % c->kv_heads) return ERR_INVALID_ARG;
-    if (q_heads > 65536 || c->pages * c->kv_heads * c->page_size > INT32_MAX) return ERR_BOUNDS;
+    if (q_heads > 65536 || c->pages > (uint64_t)INT32_MAX / (c->kv_heads * c->page_size)) return ERR_BOUNDS;
     return OK;
 }
 

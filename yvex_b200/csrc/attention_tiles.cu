@@ -13,6 +13,11 @@
 // The running maximum is only followed when it grows by more than kSlack powers of two: rescaling O means reading and writing it back, and a
 // weight of up to 2^kSlack costs no precision in f32 sums. f16 weights are lifted by 2^10 so that small ones do not
 // become subnormal, and follow the maximum sooner.
+//
+// A block of 128 keys for two tiles takes 2900 to 3100 cycles, of which the tensor cores work 2048 and the exponentials (16 a cycle and SM) as much:
+// what is left is that S and PV stand behind one another in the tensor cores' queue and that there is one buffer of S for two streams. 16 trees of
+// 32 to 64 nodes over 100 to 32768 keys (32 query heads, 8 kv heads, 128 dims, 1.02 GB of cache): 265 us, 3.9 TB/s; chunks of two prompts (573
+// GFLOP): 550 us, 1.04 PFLOP/s.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -90,7 +95,7 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     if (smem_u32(smem_raw) & 1023u) {                           // uniform: nothing has been set up yet
         pdl_wait();
-        if (threadIdx.x == 0) raise(p.status, YVEX_B200_STATUS_TIMEOUT);
+        if (threadIdx.x == 0) { raise(p.status, YVEX_B200_STATUS_TIMEOUT); p.share[blockIdx.x].rows = 0; }
         return;
     }
     uint8_t *q_tiles = smem_raw, *k_tiles = q_tiles + NS * kQBytes, *v_tiles = k_tiles + kStages * kTileBytes;
