@@ -433,6 +433,61 @@ def test_attention_pages_past_32_bits(L, fresh):
     check_attention(s, out, q, k[at], v[at])
 
 
+@pytest.mark.parametrize("group", [32, 128, 130, 256])
+@pytest.mark.parametrize("fresh", [1, 3])
+def test_attention_large_groups(L, fresh, group):
+    """Groups of which a tile holds several tokens, one, a token and a part, and half a token."""
+    s = Step(L, [200, 7], [fresh, 1], 16, extra_tokens=1)
+    out, q, k, v, _ = attend(L, s, 1, group, 64, "bfloat16")
+    assert s.status.read() == 0
+    check_attention(s, out, q, k, v)
+
+
+@pytest.mark.parametrize("fresh", [1, 20])
+def test_attention_of_shared_pages(L, fresh):
+    """Requests whose tables begin with the same pages: a common prefix, stored once."""
+    import torch
+    s = Step(L, [160, 160, 96], [fresh, fresh, fresh], 32, extra_pages=9)
+    for r in (1, 2):
+        s.table[r, :3] = s.table[0, :3]
+    s.table_dev.copy_(ints(s.table))
+    out, q, k, v, _ = attend(L, s, 2, 4, 128, "float16")
+    assert s.status.read() == 0
+    check_attention(s, out, q, k, v)
+
+
+@pytest.mark.parametrize("fresh,tree", [(5, None), (40, "random")])
+def test_attention_behind_other_kernels(L, fresh, tree):
+    """Plan, append and attention of many steps in flight on one stream, each writing what the next one reads, with nothing waited for
+    between them: the last step's results are those of the same steps one at a time."""
+    import torch
+    def go(wait):
+        s = Step(L, [0, 0], [fresh, fresh], 16, tree=tree, extra_pages=90, extra_width=30)
+        gen = torch.Generator(device="cuda")
+        gen.manual_seed(5)
+        k, v = (torch.zeros((s.pages, 2, 16, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        cache, geometry, outs = L.kv_cache_of(k, v), L.kv_geometry_of(s.pages, 16), []
+        s.step.longest = 16 * s.width
+        ws, used, rows = L.attention_paged_workspace(cache, s.step, 8), torch.empty(1, dtype=torch.int32, device="cuda"), torch.empty((s.tokens, 2, 2, 64), device="cuda")
+        q = torch.empty((s.tokens, 8, 64), dtype=torch.bfloat16, device="cuda")
+        free = s.free_dev
+        for i in range(8):
+            rows.normal_(generator=gen)
+            q.normal_(generator=gen)
+            L.kv_plan(geometry, s.step, free, s.status, used)
+            L.kv_append(cache, s.step.slots_tensor, rows[:, 0], rows[:, 1], s.status)
+            outs.append(L.attention_paged(cache, s.step, q, 0.125, s.status, workspace=ws))
+            before, after = up(fresh * i, 16), up(fresh * (i + 1), 16)
+            free = free[2 * (after - before):].contiguous()
+            s.cached_dev += fresh
+            if wait:
+                torch.cuda.synchronize()
+        assert s.status.read() == 0
+        return outs
+    for a, b in zip(go(False), go(True)):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
 @pytest.mark.parametrize("position", [0, 777, 1499])
 def test_attention_of_a_contiguous_cache(L, position):
     """One page per session is the cache that attention_gqa_decode reads: the same values, once rounded."""

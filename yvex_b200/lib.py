@@ -523,10 +523,15 @@ def attention_f32(q, keys, values, position, scale, causal, status):
 INVALID_ARG, UNSUPPORTED = -10, -5
 
 
+_qtypes = {}
+
+
 def _qtype_of(t, where):
     """GGUF id of a tensor's type (F32, F16, BF16)."""
-    torch = _torch()
-    q = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}.get(t.dtype)
+    if not _qtypes:
+        torch = _torch()
+        _qtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
+    q = _qtypes.get(t.dtype)
     if q is None:
         raise YvexError(UNSUPPORTED, where)
     return q
