@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
         const uint32_t nowhere = (uint32_t)(p.pages * p.kv_heads * p.page_size);      // a row past the cache: the box is filled with zeros
         const uint32_t groups = (uint32_t)box_keys / 16u, page_size = (uint32_t)p.page_size;
         bool ok = true, bad_page = false;
-        uint32_t it = 0, k_asked = 0;
+        uint32_t it = 0, k_asked = 0, v_asked = 0;
         for (; w.live() && ok; w.next(p)) {
             const uint32_t end = w.q.n.cached + w.q.n.fresh;
             const int32_t *table = p.block_table + (uint64_t)w.request * p.table_width;
@@ -406,37 +406,47 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                 none = page < 0 || (uint64_t)page >= p.pages;
                 return none ? nowhere : ((uint32_t)page * p.kv_heads + w.head) * page_size + key % page_size;
             };
-            bool none, none_next;
-            uint32_t y = row_of(0, none);
-            for (uint32_t j = 0; j < w.count && ok; ++j, ++it) {
-                const uint32_t y_next = row_of(j + 1, none_next), s = it % kStages, ph = (it / kStages) & 1u;
-                bad_page |= none;
-                const uint32_t bad = __reduce_or_sync(0xffffffffu, none ? ((1u << groups) - 1u) << (groups * lane) : 0u);
-                ok = mbar_wait_warp(&sm->k_empty[s], ph ^ 1u, abort);
-                if (!ok) break;
-                if (lane == 0) { sm->bad_keys[it % Plan::kBadRing] = bad; mbar_expect_tx(&sm->k_full[s], kTileBytes); }
-                __syncwarp();
-                if (lane < boxes)
-                    for (int h = 0; h < kHalves; ++h)
-                        tma_load_2d(k_tiles + s * kTileBytes + h * BK * 128 + lane * box_keys * 128, &maps.k, 64 * h, (int)y, &sm->k_full[s]);
-                k_asked = it + 1;
-                ok = mbar_wait_warp(&sm->v_empty[s], ph ^ 1u, abort);
-                if (!ok) break;
-                if (lane == 0) mbar_expect_tx(&sm->v_full[s], kTileBytes);
-                __syncwarp();
-                if (lane < boxes)
-                    for (int h = 0; h < kHalves; ++h)
-                        tma_load_2d(v_tiles + s * kTileBytes + h * BK * 128 + lane * box_keys * 128, &maps.v, 64 * h, (int)y, &sm->v_full[s]);
-                y = y_next;
-                none = none_next;
+            // K a block ahead of V, which waits for products that come later
+            auto copy = [&](uint8_t *tiles, const CUtensorMap *map, uint32_t s, uint32_t y, uint64_t *full) {
+                if (lane >= boxes) return;
+                for (int h = 0; h < kHalves; ++h) tma_load_2d(tiles + s * kTileBytes + h * BK * 128 + lane * box_keys * 128, map, 64 * h, (int)y, full);
+            };
+            uint32_t y = 0;
+            bool none;
+            uint32_t y_next = row_of(0, none);
+            for (uint32_t j = 0; j <= w.count && ok; ++j) {
+                if (j < w.count) {                              // K of block j
+                    const uint32_t at = it + j, s = at % kStages;
+                    bad_page |= none;
+                    const uint32_t bad = __reduce_or_sync(0xffffffffu, none ? ((1u << groups) - 1u) << (groups * lane) : 0u);
+                    ok = mbar_wait_warp(&sm->k_empty[s], ((at / kStages) & 1u) ^ 1u, abort);
+                    if (!ok) break;
+                    if (lane == 0) { sm->bad_keys[at % Plan::kBadRing] = bad; mbar_expect_tx(&sm->k_full[s], kTileBytes); }
+                    __syncwarp();
+                    copy(k_tiles, &maps.k, s, y_next, &sm->k_full[s]);
+                    k_asked = at + 1;
+                }
+                const uint32_t y_now = y_next;
+                if (j < w.count) y_next = row_of(j + 1, none);
+                if (j) {                                        // V of the block before
+                    const uint32_t at = it + j - 1, s = at % kStages;
+                    ok = mbar_wait_warp(&sm->v_empty[s], ((at / kStages) & 1u) ^ 1u, abort);
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(&sm->v_full[s], kTileBytes);
+                    __syncwarp();
+                    copy(v_tiles, &maps.v, s, y, &sm->v_full[s]);
+                    v_asked = at + 1;
+                }
+                y = y_now;
             }
+            it += w.count;
         }
         if (bad_page) raise(p.status, YVEX_B200_STATUS_ARGUMENT);
         if (!ok && lane == 0) {
             // copies in flight must land before the CTA's shared memory is someone else's
             volatile int none = 0;
             for (uint32_t i = k_asked > kStages ? k_asked - kStages : 0; i < k_asked; ++i) mbar_wait(&sm->k_full[i % kStages], (i / kStages) & 1u, &none);
-            for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_wait(&sm->v_full[i % kStages], (i / kStages) & 1u, &none);
+            for (uint32_t i = v_asked > kStages ? v_asked - kStages : 0; i < v_asked; ++i) mbar_wait(&sm->v_full[i % kStages], (i / kStages) & 1u, &none);
         }
         __syncwarp();
     } else if (warp == Plan::kSoftmaxWarps + 1) {
