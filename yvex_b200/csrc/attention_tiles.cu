@@ -16,8 +16,8 @@
 //
 // A block of 128 keys for two tiles takes 2900 to 3100 cycles, of which the tensor cores work 2048 and the exponentials (16 a cycle and SM) as much:
 // what is left is that S and PV stand behind one another in the tensor cores' queue and that there is one buffer of S for two streams. 16 trees of
-// 32 to 64 nodes over 100 to 32768 keys (32 query heads, 8 kv heads, 128 dims, 1.02 GB of cache): 265 us, 3.9 TB/s; chunks of two prompts (573
-// GFLOP): 550 us, 1.04 PFLOP/s.
+// 32 to 64 nodes over 100 to 32768 keys (32 query heads, 8 kv heads, 128 dims, 1.02 GB of cache): 270 us, 3.8 TB/s; chunks of two prompts (573
+// GFLOP): 585 us, 0.98 PFLOP/s (307 and 592 with three sets of inputs in rotation).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
