@@ -1,0 +1,57 @@
+"""The serving step's Python front end and refusals at their edges (no GPU)."""
+import gc
+import weakref
+from types import SimpleNamespace as N
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def L():
+    from yvex_b200 import build
+    build.build()
+    from yvex_b200 import lib
+    return lib
+
+
+@pytest.fixture
+def front(L, monkeypatch):
+    """The front end over a library that takes every call, with host tensors standing in for a device's."""
+    import torch
+    monkeypatch.setattr(L, "_torch", lambda: torch)
+    monkeypatch.setattr(L, "_device", lambda: -1)
+    monkeypatch.setattr(L, "_on", lambda dev: None)
+    monkeypatch.setattr(L, "lib", N(**{"yvex_b200_" + n: lambda *a: 0 for n in ("kv_plan", "kv_append", "attention_paged", "logits_edit")}))
+    return L
+
+
+def i32(*shape):
+    import torch
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def status():
+    return N(word=i32(1))
+
+
+def cache_and_step(L):
+    import torch
+    k = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    return L.kv_cache_of(k, k), L.kv_step_of(i32(3), i32(3), i32(3, 5), tokens=7, longest_fresh=3, longest=50)
+
+
+def test_a_step_keeps_what_a_captured_call_writes(front):
+    """A captured plan or attention goes on using the count and the workspace that it was given: they live as long as the step's description,
+    also where the caller's names for them are used again."""
+    import torch
+    c, s = cache_and_step(front)
+    used, ws, q = i32(1), torch.zeros(64, dtype=torch.uint8), torch.zeros((7, 8, 64), dtype=torch.bfloat16)
+    front.kv_plan(c, s, i32(3), status(), used)
+    front.attention_paged(c, s, q, 0.1, status(), workspace=ws)
+    refs = [weakref.ref(used), weakref.ref(ws)]
+    del used, ws
+    gc.collect()
+    assert all(r() is not None for r in refs)
+    del s
+    gc.collect()
+    assert all(r() is None for r in refs)

@@ -612,12 +612,14 @@ def kv_step_of(cached, fresh, block_table, tokens, longest_fresh, longest, paren
 
 
 def kv_plan(cache, step, free_pages, status, pages_used=None):
-    """Plans the step on the device (see yvex_b200_kv_plan); free_pages int32 -> pages_used [1] int32, how many of them it took."""
+    """Plans the step on the device (see yvex_b200_kv_plan); free_pages int32 -> pages_used [1] int32, how many of them it took. (The step
+    keeps the last pages_used, and the workspace that attention_paged was given: a captured call goes on writing them.)"""
     torch, dev = _torch(), _device()
     if pages_used is None:
         pages_used = torch.empty(1, dtype=torch.int32, device=free_pages.device)
     _check(lib.yvex_b200_kv_plan(cache, step, _array(free_pages, torch.int32, None, "kv_plan", dev), free_pages.numel(),
                                  _array(pages_used, torch.int32, 1, "kv_plan", dev), status.word.data_ptr(), _on(dev)), "kv_plan")
+    step.used_tensor = pages_used
     return pages_used
 
 
@@ -647,6 +649,8 @@ def attention_paged(cache, step, q, scale, status, workspace=None, out=None):
     heads = shape[1]
     if workspace is None:
         workspace = attention_paged_workspace(cache, step, heads)
+    else:
+        step.workspace_tensor = workspace
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=q.device)
     _check(lib.yvex_b200_attention_paged(cache, step, q.data_ptr(), _row_stride(q, w), heads, scale, _array(out, dtype, q.numel(), w, dev),
