@@ -158,15 +158,19 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
     uint16_t *list = reinterpret_cast<uint16_t *>(counters + slots);
     const uint64_t first_row = (uint64_t)blockIdx.x * a.rows_per_cta, last_row = min(a.d.rows, first_row + a.rows_per_cta);
     bool bad_arg = false, bad_num = false, waited = false;
-    uint32_t parts = gridDim.y, part = blockIdx.y;      // words w with hash(w) % parts == part are in the table
+    uint32_t parts = gridDim.y, part = blockIdx.y;      // words of that part are in the table
 
-    auto hash = [](int32_t w) { return (uint32_t)w * 0x9E3779B1u; };
+    auto hash = [](uint32_t w) { return w * 0x9E3779B1u; };
+    // Parts nest: of a power of two of them, part p falls into 2p and 2p + 1 of twice as many, whatever the words are. The high bits of a
+    // second hash say which, so that neither a step between the words (their low bits alone make the low bits of the first) nor
+    // the place in the table, which the first one's high bits give, tells the part.
+    auto part_of = [&](uint32_t h) { return __umulhi(hash(h ^ (h >> 15)), parts); };
     // The slot of word w, which is entered if it is not there; -1 for padding, words of other parts, and when the table is full.
     auto slot_of = [&](int32_t w) -> int {
         if (w < 0) return -1;
         if ((uint32_t)w >= vocabulary) { bad_arg = true; return -1; }
-        const uint32_t h = hash(w);
-        if ((h & (parts - 1u)) != part) return -1;
+        const uint32_t h = hash((uint32_t)w);
+        if (parts != 1u && part_of(h) != part) return -1;
         uint32_t s = h >> (32u - a.table_log2);
         for (uint32_t tries = 0; tries < slots; ++tries, s = (s + 1u) & (slots - 1u)) {
             uint32_t k = *(volatile uint32_t *)&keys[s];
@@ -309,7 +313,7 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
                     __syncthreads();
                 }
             }
-            // the next part: the sibling, or the one that follows the last parent that is done
+            // the next part: the other half of the one that was split, or what follows once both are done
             ++part;
             while (parts > gridDim.y && !(part & 1u)) { part >>= 1; parts >>= 1; }
             if (parts == gridDim.y) break;
