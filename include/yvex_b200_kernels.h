@@ -480,7 +480,8 @@ typedef struct yvex_b200_kv_step {
  * Entries of block_table below ceil(cached / page_size) are read, others are left alone. Padding rows get slot and
  * request -1, position and mask 0. Of `cache` only pages and page_size are read. Status 2: a negative length, one above its bound, more rows
  * than `tokens`, more pages than free_count or table_width, a page id outside the cache, a parent not below its
- * child: the rows concerned get slot -1 (a bad parent counts as -1), the others are planned.
+ * child: the rows concerned get slot -1 (a bad parent counts as -1), the others are planned. All rows of a request with a bad length are
+ * concerned; it takes no pages and its row of block_table stays as it was.
  */
 int yvex_b200_kv_plan(const yvex_b200_kv_cache *cache, const yvex_b200_kv_step *step, const int32_t *free_pages,
                       uint64_t free_count, int32_t *pages_used, int *status, void *stream);
@@ -499,7 +500,7 @@ int yvex_b200_kv_append(const yvex_b200_kv_cache *cache, const int64_t *slots, u
  * sees no key (an empty mask over an empty cache) is zero; padding rows of out are left as they were. Keys that a row does
  * not see have no influence on it, whatever is stored there. Of the step's arrays cached, block_table, offsets and ancestors
  * (trees) are read. Status 1: an output that is not finite; 2: lengths above their bounds, offsets that are not those of a
- * plan, a page id outside the cache (its keys then count as unseen). workspace: yvex_b200_attention_paged_workspace_bytes of the same cache
+ * plan (the rows of such a request are left as they were), a page id outside the cache (its keys then count as unseen). workspace: yvex_b200_attention_paged_workspace_bytes of the same cache
  * and step bounds, 16-byte aligned; calls that may overlap in time need one each.
  */
 uint64_t yvex_b200_attention_paged_workspace_bytes(const yvex_b200_kv_cache *cache, const yvex_b200_kv_step *step, uint64_t q_heads);

@@ -52,3 +52,63 @@ def test_logits_words_that_do_not_fit_a_table(L, rows, name, where):  # noqa: F8
     check_edit(out, want, [0] * rows, out)
     L.logits_edit(policy, drafts, x, st, out=x)
     assert st.read() == 0 and torch.equal(x, out)
+
+
+# ---- plan: requests whose lengths are bad -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tree", [None, "random"])
+@pytest.mark.parametrize("change", ["negative_cached", "fresh_above_its_bound", "sum_above_its_bound", "far"])
+def test_plan_leaves_requests_with_bad_lengths_alone(L, change, tree):  # noqa: F811
+    """Rows of a request with a negative length or one above its bound get no slot, and the request no pages and no table entries; the others
+    are planned as if it brought no pages, and the rows behind it lie where its fresh tokens leave them."""
+    import torch
+    cached, fresh = [20, 30, 33], [3, 4, 5]
+    s = Step(L, cached, fresh, 16, tree=tree, extra_tokens=9)
+    s.step.longest_fresh, s.step.longest = 5, 38
+    if change == "negative_cached":
+        s.cached_dev[1] = -1
+        n, position = 4, 0
+    elif change == "fresh_above_its_bound":
+        s.fresh_dev[1] = 6                                       # (and 30 + 6 is within `longest`)
+        n, position = 6, 30
+    elif change == "sum_above_its_bound":
+        s.cached_dev[1] = 35                                     # 35 + 4: one more than `longest`
+        n, position = 4, 35
+    else:
+        s.cached_dev[1] = 2 ** 31 - 1
+        n, position = 4, 2 ** 31 - 1
+    if tree:                                                     # parents of rows that moved: children of the cache
+        s.step._keep[2][3:].fill_(-1)
+    before = s.table_dev.clone()
+    used = s.plan()
+    assert s.status.read() == 2
+    held = s.table
+    want = [int(held[0, 1]) * 16 + 4 + i for i in range(3)] + [-1] * n
+    free = s.free.tolist()
+    # request 0 stays in its page; request 2 has 33 tokens in three pages: 34 .. 38 stay there too
+    want += [int(held[2, 2]) * 16 + 1 + i for i in range(5)]
+    want += [-1] * (s.tokens - len(want))
+    assert s.step.slots_tensor.tolist() == want
+    assert s.step.offsets_tensor.tolist() == [0, 3, 3 + n, 8 + n] and used.tolist() == [0]
+    assert s.step.row_request_tensor.tolist() == [0] * 3 + [1] * n + [2] * 5 + [-1] * (s.tokens - 8 - n)
+    assert torch.equal(s.table_dev, before) and free == s.free_dev.tolist()
+    if not tree:
+        assert s.step.positions_tensor.tolist()[3:3 + n] == [min(position + i, 2 ** 31 - 1) for i in range(n)]
+
+
+def test_plan_counts_pages_of_good_requests_only(L):  # noqa: F811
+    """Pages of the requests around a bad one are those that they would get without it."""
+    for bad in ([-7, 4], [60, 5], [10, 60]):
+        s = Step(L, [14, 10, 30, 1], [4, 5, 4, 3], 16, extra_tokens=60)
+        s.step.longest_fresh, s.step.longest = 5, 64
+        free = s.free.tolist()
+        s.cached_dev[1], s.fresh_dev[1] = bad
+        used = s.plan()
+        assert s.status.read() == 2 and used.tolist() == [2]
+        table, f = s.table_dev.cpu().numpy(), bad[1]
+        assert [table[0, 1], table[2, 2]] == free[:2]
+        slots = s.step.slots_tensor.tolist()
+        assert slots[4:4 + f] == [-1] * f
+        page = lambda r, n: int(table[r, n // 16]) * 16 + n % 16  # noqa: E731
+        assert slots[:4] == [page(0, 14 + i) for i in range(4)] and slots[4 + f:8 + f] == [page(2, 30 + i) for i in range(4)]
+        assert slots[8 + f:11 + f] == [page(3, 1 + i) for i in range(3)]

@@ -40,6 +40,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanParams 
     int request = -1;
     bool bad = false;
 
+    // Lengths that no step can have: the request's rows get no slot and the request no pages.
+    auto impossible = [&](int32_t cs, int32_t fs) {
+        return cs < 0 || fs < 0 || (uint64_t)fs > p.longest_fresh || (uint64_t)cs + (uint64_t)fs > p.longest || (p.tree && fs > kPlanHalo);
+    };
+
     pdl_trigger();
     pdl_wait();
     int parent = -1;
@@ -47,13 +52,15 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanParams 
     for (uint64_t chunk = 0; chunk < p.requests; chunk += kPlanThreads) {
         const uint64_t r = chunk + tid;
         uint32_t c = 0, f = 0;
+        bool none = false;
         if (r < p.requests) {
             const int32_t cs = p.cached[r], fs = p.fresh[r];
-            bad |= cs < 0 || fs < 0 || (uint64_t)fs > p.longest_fresh || (uint64_t)cs + (uint64_t)fs > p.longest || (p.tree && fs > kPlanHalo);
+            none = impossible(cs, fs);
+            bad |= none;
             c = cs < 0 ? 0u : (uint32_t)cs;
             f = fs < 0 ? 0u : (uint32_t)fs;
         }
-        const uint32_t need = (uint32_t)(((uint64_t)c + f + S - 1) / S) - (uint32_t)(((uint64_t)c + S - 1) / S);
+        const uint32_t need = none ? 0u : (uint32_t)(((uint64_t)c + f + S - 1) / S) - (uint32_t)(((uint64_t)c + S - 1) / S);
         int64_t rows = f, pages = need;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -124,11 +131,12 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanParams 
         int64_t slot = -1;
         int32_t position = 0;
         if (request >= 0) {
-            const uint32_t c = (uint32_t)max(p.cached[request], 0);
+            const int32_t cs = p.cached[request];
+            const uint32_t c = (uint32_t)max(cs, 0);
             const uint64_t at = (uint64_t)c + (uint64_t)index, col = at / S;
             const uint64_t held = ((uint64_t)c + S - 1) / S;
             int32_t page = -1;
-            if (col < p.table_width) {
+            if (col < p.table_width && !impossible(cs, p.fresh[request])) {
                 int32_t *entry = p.block_table + (uint64_t)request * p.table_width + col;
                 if (col < held) {
                     page = *entry;
