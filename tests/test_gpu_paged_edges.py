@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import paged_oracle as O
-from test_gpu_paged import L, Step, check_attention, check_edit, ints, up  # noqa: F401
+from test_gpu_paged import L, Step, attend, check_attention, check_edit, ints, up  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +112,28 @@ def test_plan_counts_pages_of_good_requests_only(L):  # noqa: F811
         page = lambda r, n: int(table[r, n // 16]) * 16 + n % 16  # noqa: E731
         assert slots[:4] == [page(0, 14 + i) for i in range(4)] and slots[4 + f:8 + f] == [page(2, 30 + i) for i in range(4)]
         assert slots[8 + f:11 + f] == [page(3, 1 + i) for i in range(3)]
+
+
+# ---- attention: weights far below the largest -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("group", [2, 12])
+@pytest.mark.parametrize("above", [8, 12, 15, 16, 17, 20])
+def test_attention_one_key_far_above_the_others(L, above, group, dtype):  # noqa: F811
+    """A key (one for each 16 of a block of 64) whose score is `above` nats over two thousand others and whose value is zero: what is left is the
+    others' weights, e^-above each, which f16 would hold with few bits or none beside a weight of one. The bound counts half a
+    step of every weight."""
+    import torch
+    s = Step(L, [2000] * 64, [1] * 64, 16)
+    _, q, k, v, cache = attend(L, s, 8, group, 64, dtype)
+    q.zero_()
+    q[..., 0] = 1
+    k.zero_()
+    v.fill_(1000)
+    for j in range(0, 64, 16):
+        page = ints(s.table[:, j // 16]).long()
+        k[page, :, j % 16, 0], v[page, :, j % 16] = above, 0
+    out = torch.full_like(q, 7.0)
+    L.attention_paged(cache, s.step, q, 1.0, s.status, out=out)
+    assert s.status.read() == 0
+    check_attention(s, out, q, k, v, 1.0)

@@ -5,7 +5,9 @@
 // mma.sync m16n8k16 with operands built from 16-byte loads as they lie in memory (the k-slots of S are whatever dims, those
 // of PV whatever keys a lane holds), so nothing is staged or transposed. 16 keys never straddle a page, and the page
 // of a warp's next block is looked up while this one is computed. The weights are rounded once to the cache's type for the second product,
-// which adds less to the output's error than its own rounding (an output of f32 would not allow that); their sum stays f32 and unrounded.
+// which adds less to the output's error than its own rounding (an output of f32 would not allow that); their sum stays f32 and unrounded. f16
+// weights are lifted by 2^15 before, and their sums with them, so that those down to 2^-29 of the largest keep all their bits and smaller ones are off by at
+// most 2^-40 of it: of a million keys that is 2^-20 (unlifted, the many small weights beside one large key were lost: 2^-25 each).
 // 64 sessions of 100 to 32768 keys (3.46 GB): 558 us, 6.2 TB/s, 94 % of the copy bandwidth; equal shares of blocks instead of a fixed number of
 // slices per session are what holds that for ragged lengths. One session of 1500 keys: 12 us for the two kernels, all latency.
 #include <cuda_bf16.h>
@@ -49,6 +51,7 @@ __global__ void __launch_bounds__(kRowsThreads, R == 8 && D <= 128 ? 3 : 2) page
     PagedWalk<R, kRowsBlock, kRowsCost> w;
     const uint32_t units_per_page = (uint32_t)(p.page_size / 16);
     const float scale = p.scale * 1.4426950408889634f;          // scores in powers of two
+    constexpr float kLift = std::is_same<T, __half>::value ? 32768.0f : 1.0f;
     if (tid == 0) p.share[blockIdx.x].rows = 0;
     bool bad_page = false, bad_out = false;
 
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(kRowsThreads, R == 8 && D <= 128 ? 3 : 2) page
                 }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const float p0 = exp2f(x[half][0] - shift), p1 = exp2f(x[half][1] - shift);
+                    const float p0 = exp2f(x[half][0] - shift) * kLift, p1 = exp2f(x[half][1] - shift) * kLift;     // (exact)
                     pa[half][h] = close2<T>(p0, p1);
                     l[h] += p0 + p1;
                 }
