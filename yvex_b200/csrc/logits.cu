@@ -2,8 +2,8 @@
 //
 // Two kernels. The first streams the rows through with nothing but the grammar's mask: bound by HBM (8 bytes a word for f32 rows). The
 // second edits the words that occur in a request's history, on a row's path or among its biases, a few in a hundred, in place: a CTA
-// takes several rows of a request, counts its words in a hash table in shared memory (key, and one 32-bit counter: bit 31 occurs in the
-// prompt, bit 30 has a bias, the rest how often it was generated), and then visits the table's words for every row. The table is built while the
+// takes several rows of a request, counts its words in a hash table in shared memory (key, one 32-bit counter: bit 31 occurs in the
+// prompt, the rest how often it was generated, and, where there are biases, the last entry of the word), and then visits the table's words for every row. The table is built while the
 // stream runs. Counters are integers, so the order of the atomics does not show. Requests with more words than the table holds are done in
 // parts of the words, halved until they fit. (One kernel with counters for a share of the vocabulary and the edits in the stream took 204 us for
 // 419 rows of 129280 words, with the edits behind the stream 175: nearly every warp meets a counted word among its 128, and every share
@@ -14,8 +14,8 @@
 namespace yb {
 
 constexpr int kStreamThreads = 256, kStreamLoads = 4, kStreamCtas = 4;      // of the stream: loads of 16 bytes, CTAs an SM
-constexpr int kEditThreads = 1024, kEditsAhead = 4, kBiases = 256;       // of the edits: words a thread has on their way, bias entries that a CTA lists
-constexpr uint32_t kSeen = 1u << 31, kBiased = 1u << 30, kCount = kBiased - 1u;
+constexpr int kEditThreads = 1024, kEditsAhead = 4;       // of the edits: words a thread has on their way
+constexpr uint32_t kSeen = 1u << 31, kCount = kSeen - 1u;
 constexpr uint32_t kLeastTable = 1024, kMostTable = 16384;
 
 struct LogitsParams {
@@ -149,13 +149,14 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamCtas) logits_stream_ker
 // blockIdx.x: the rows, blockIdx.y of gridDim.y (a power of two): the words.
 template <class T>
 __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsParams a) {
-    extern __shared__ __align__(16) uint32_t keys[];    // words (~0: none), their counters, the list of those in use
-    __shared__ int2 biases[kBiases];                    // bias entries: slot of the word, index of the entry
-    __shared__ int bias_count, list_count;
+    extern __shared__ __align__(16) uint32_t keys[];    // words (~0: none), their counters, the list of those in use, the last bias entries (-1: none)
+    __shared__ int list_count;
     const int tid = threadIdx.x;
     const uint32_t slots = 1u << a.table_log2, limit = slots / 4 * 3, vocabulary = (uint32_t)a.p.vocabulary;
     uint32_t *counters = keys + slots;
     uint16_t *list = reinterpret_cast<uint16_t *>(counters + slots);
+    int *last_bias = reinterpret_cast<int *>(list + slots);
+    const bool biased = a.p.bias_tokens != nullptr;
     const uint64_t first_row = (uint64_t)blockIdx.x * a.rows_per_cta, last_row = min(a.d.rows, first_row + a.rows_per_cta);
     bool bad_arg = false, bad_num = false, waited = false;
     uint32_t parts = gridDim.y, part = blockIdx.y;      // words of that part are in the table
@@ -227,7 +228,8 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
             __syncthreads();
             for (uint32_t i = tid; i < slots / 2; i += kEditThreads)
                 reinterpret_cast<uint4 *>(keys)[i] = i < slots / 4 ? make_uint4(~0u, ~0u, ~0u, ~0u) : make_uint4(0, 0, 0, 0);
-            if (tid == 0) { bias_count = 0; list_count = 0; }
+            for (uint32_t i = tid; biased && i < slots / 4; i += kEditThreads) reinterpret_cast<int4 *>(last_bias)[i] = make_int4(-1, -1, -1, -1);
+            if (tid == 0) list_count = 0;
             __syncthreads();
             for (int64_t t0 = from + tid; t0 < to; t0 += 4 * kEditThreads) {
                 int32_t w[4];                           // (four words on their way at a time)
@@ -243,10 +245,7 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
             }
             for (int64_t t = bias_from + tid; t < bias_to; t += kEditThreads) {
                 const int s = slot_of(a.p.bias_tokens[t]);
-                if (s < 0) continue;
-                atomicOr(&counters[s], kBiased);
-                const int n = atomicAdd(&bias_count, 1);
-                if (n < kBiases) biases[n] = make_int2(s, (int)t);
+                if (s >= 0) atomicMax(&last_bias[s], (int)t);
             }
             // drafted words have their slots before the first row; a tree's nodes keep a thread each
             int node = -1;
@@ -278,7 +277,7 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
                     for (int q = 0; q < kEditsAhead; ++q) {     // (in place, the stream has left the words as they were, or -inf where the grammar forbids them)
                         const int i = i0 + q * kEditThreads;
                         slot[q] = i < n ? list[i] : -1;
-                        if (slot[q] >= 0 && !counters[slot[q]]) slot[q] = -1;
+                        if (slot[q] >= 0 && !counters[slot[q]] && !(biased && last_bias[slot[q]] >= 0)) slot[q] = -1;
                         if (slot[q] >= 0) x[q] = LogitsVec<T>::get(in + keys[slot[q]]);
                     }
 #pragma unroll
@@ -287,19 +286,12 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
                         if (s < 0) continue;
                         const uint32_t c = counters[s], word = keys[s], times = c & kCount;
                         float y = x[q];
-                        if (c & (kSeen | kCount)) {
+                        if (c) {
                             y = y > 0.0f ? y / rep : y * rep;
                             if (times) y -= frequency * (float)times + presence;
                         }
-                        if (c & kBiased) {              // the last entry of a word counts
-                            int last = -1;
-                            if (bias_count <= kBiases) {
-                                for (int b = 0; b < bias_count; ++b) if (biases[b].x == s) last = max(last, biases[b].y);
-                            } else {                    // more than the list holds
-                                for (int64_t b = bias_to - 1; b >= bias_from && last < 0; --b) if ((uint32_t)a.p.bias_tokens[b] == word) last = (int)b;
-                            }
-                            y += a.p.bias_values[last];
-                        }
+                        const int last = biased ? last_bias[s] : -1;      // the last entry of a word counts
+                        if (last >= 0) y += a.p.bias_values[last];
                         if (!allows(allowed, word)) y = -INFINITY;
                         bad_num |= y != y;
                         LogitsVec<T>::put(out + word, y);
@@ -338,8 +330,9 @@ template <class T> static int launch_logits(LogitsParams &a, cudaStream_t s) {
     uint32_t slots = kLeastTable;
     a.table_log2 = 10;
     while (slots < 2 * words && slots < kMostTable) { slots *= 2; ++a.table_log2; }
-    constexpr uint64_t per_slot = 2 * sizeof(uint32_t) + sizeof(uint16_t);
-    const int rc = optin.ensure(logits_edit_kernel<T>, (int)(kMostTable * per_slot));
+    constexpr uint64_t per_word = 2 * sizeof(uint32_t) + sizeof(uint16_t);
+    const uint64_t per_slot = per_word + (a.p.bias_tokens ? sizeof(int) : 0);
+    const int rc = optin.ensure(logits_edit_kernel<T>, (int)(kMostTable * (per_word + sizeof(int))));
     if (rc != OK) return rc;
     uint64_t parts = 1;
     while (a.d.rows * parts * 2 <= kSmCount && parts * 128 < words) parts *= 2;
