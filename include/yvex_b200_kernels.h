@@ -522,7 +522,7 @@ int yvex_b200_attention_paged(const yvex_b200_kv_cache *cache, const yvex_b200_k
  * request out of range, offsets that decrease or pass the packed arrays' lengths, a repetition that is not positive and finite (it counts as 1).
  */
 typedef struct yvex_b200_logits_policy {
-    uint64_t vocabulary, requests, history_tokens, bias_entries;    /* the last two: lengths of the packed arrays */
+    uint64_t vocabulary, requests, history_tokens, bias_entries;    /* the last two: lengths of the packed arrays; history and rows together below 2^31 */
     const int32_t *history, *history_offsets, *prompt_lengths;
     const float *repetition, *presence, *frequency;
     const int32_t *bias_tokens;

@@ -354,6 +354,7 @@ extern "C" int yvex_b200_logits_edit(const yvex_b200_logits_policy *p, const yve
     if (qtype != Q_F32 && qtype != Q_F16 && qtype != Q_BF16) return ERR_UNSUPPORTED;
     if (p->vocabulary > INT32_MAX || p->requests >= INT32_MAX || d->rows >= INT32_MAX || p->history_tokens > INT32_MAX || p->bias_entries > INT32_MAX)
         return ERR_BOUNDS;
+    if (p->history_tokens > (uint64_t)kCount - d->rows) return ERR_BOUNDS;      // (a word's counter has 31 bits, for the history and a path)
     if (logits_stride < p->vocabulary || out_stride < p->vocabulary || (grammar && grammar_stride < (p->vocabulary + 31) / 32)) return ERR_BOUNDS;
     if ((p->history && !p->history_offsets) || (p->bias_tokens && (!p->bias_values || !p->bias_offsets))) return ERR_INVALID_ARG;
     if (!d->row_request && d->rows > p->requests) return ERR_BOUNDS;
