@@ -55,3 +55,13 @@ def test_a_step_keeps_what_a_captured_call_writes(front):
     del s
     gc.collect()
     assert all(r() is None for r in refs)
+
+
+def test_histories_that_a_counter_cannot_count_are_refused(L):
+    """A word's counter has 31 bits, for what occurs in the history and on a path of drafted words."""
+    P, before = 0x10000, L.lib.yvex_b200_launch_count()
+    drafts = L.LogitsDrafts(9, 0, P, P, P)
+    for tokens in (2 ** 31 - 9, 2 ** 31 - 1):
+        policy = L.LogitsPolicy(1000, 9, tokens, 0, P, P)
+        assert L.lib.yvex_b200_logits_edit(policy, drafts, 0, P, 1000, None, 0, P, 1000, P, None) == -7
+    assert L.lib.yvex_b200_launch_count() == before
