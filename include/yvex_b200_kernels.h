@@ -518,7 +518,7 @@ int yvex_b200_attention_paged(const yvex_b200_kv_cache *cache, const yvex_b200_k
  * the bias arrays may be NULL. The drafts are those of a step: row t belongs to row_request[t] (NULL: request t; a negative one is
  * padding and its row of out is left as it was), drafted[t] is the word that was fed for row t (NULL: no paths), and the path of a row
  * are the drafted words of its ancestors and itself. Negative words are padding. logits and out have `qtype` F32, F16 or BF16 with strides in elements; out may be
- * logits. grammar: [rows] bit masks of grammar_stride words of 32 bits, NULL for none. Arithmetic is f32, rounded once. Status 1: a NaN in an allowed place; 2: a word or
+ * logits (the same rows with the same stride; rows that overlap in another way are refused). grammar: [rows] bit masks of grammar_stride words of 32 bits, NULL for none. Arithmetic is f32, rounded once. Status 1: a NaN in an allowed place; 2: a word or
  * request out of range, offsets that decrease or pass the packed arrays' lengths, a repetition that is not positive and finite (it counts as 1).
  */
 typedef struct yvex_b200_logits_policy {

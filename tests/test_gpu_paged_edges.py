@@ -78,6 +78,28 @@ def test_logits_long_bias_lists(L, rows):  # noqa: F811
     assert begin.elapsed_time(end) < (10.0 if rows == 80 else 2.0), begin.elapsed_time(end)
 
 
+def test_logits_beside_out_in_one_buffer(L):  # noqa: F811
+    """Rows of logits and of out that lie among one another without overlapping, with equal strides and different ones, and in place with a stride."""
+    import torch
+    V = 1000
+    policy, drafts, st = L.logits_policy_of(V, ints([1, 1, 7]), ints([0, 3]), frequency=ints([0.5], torch.float32)), L.logits_drafts_of(row_request=ints([0] * 5)), L.Status()
+    x = torch.randn((5, V), device="cuda")
+    want = x.clone()
+    want[:, 1] -= 1.0
+    want[:, 7] -= 0.5
+    def views(kind):
+        flat = torch.full((60000,), 9.0, device="cuda")
+        at = lambda start, stride: flat[start:].as_strided((5, V), (stride, 1), flat.storage_offset() + start)  # noqa: E731
+        return {"pairs": (at(0, 2000), at(1000, 2000)), "pairs_back": (at(1000, 2000), at(0, 2000)), "far": (at(0, 1000), at(5000, 1000)),
+                "threes": (at(0, 3000), at(2000, 6000)), "inside": (at(1000, 8000), at(2000, 1000)), "in_place": (at(3, 1234),) * 2}[kind]
+    for kind in ("pairs", "pairs_back", "far", "threes", "inside", "in_place"):
+        rows, out = views(kind)
+        rows.copy_(x)
+        L.logits_edit(policy, drafts, rows, st, out=out)
+        assert st.read() == 0 and torch.equal(out, want), kind
+        assert kind == "in_place" or torch.equal(rows, x), kind
+
+
 # ---- plan: requests whose lengths are bad -----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("tree", [None, "random"])

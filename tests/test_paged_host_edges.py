@@ -65,3 +65,19 @@ def test_histories_that_a_counter_cannot_count_are_refused(L):
         policy = L.LogitsPolicy(1000, 9, tokens, 0, P, P)
         assert L.lib.yvex_b200_logits_edit(policy, drafts, 0, P, 1000, None, 0, P, 1000, P, None) == -7
     assert L.lib.yvex_b200_launch_count() == before
+
+
+def overlap(L, rows, start, stride, out, out_stride, qtype=0, V=1000):
+    return L.lib.yvex_b200_logits_edit(L.LogitsPolicy(V, rows), L.LogitsDrafts(rows), qtype, start, stride, None, 0, out, out_stride, 0x10000, None)
+
+
+def test_logits_and_out_that_overlap_without_being_the_same_rows_are_refused(L):
+    """Rows that another row's words are written into: the same start with another stride, shifted views, one row inside another."""
+    P, before = 1 << 20, L.lib.yvex_b200_launch_count()
+    for rows, start, stride, out, out_stride, qtype in (
+            (2, P, 1000, P, 1004, 0), (2, P, 2000, P, 1000, 0), (1, P, 1000, P + 4, 1000, 0), (1, P + 16, 1000, P, 1000, 0), (3, P, 1000, P + 4000, 1000, 0),
+            (3, P + 4000, 1000, P, 1000, 0), (3, P, 2000, P + 4 * 999, 2000, 0), (3, P, 2000, P + 4 * 1001, 2000, 0), (3, P + 4 * 2999, 2000, P, 2000, 0),
+            (5, P, 2000, P + 4000, 3000, 0), (2, P, 1000, P + 2, 1000, 1), (1 << 20, P, 1000, P + 4 * 1000 * ((1 << 20) - 1), 1000, 0),
+            (4, P, 1 << 40, P + (3 << 42) + 3996, 1 << 40, 0), (9, P, 1000, P + 4 * 8999, 5000, 0)):
+        assert overlap(L, rows, start, stride, out, out_stride, qtype) == -10, (rows, start - P, stride, out - P, out_stride, qtype)
+    assert L.lib.yvex_b200_launch_count() == before

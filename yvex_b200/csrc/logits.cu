@@ -343,6 +343,23 @@ template <class T> static int launch_logits(LogitsParams &a, cudaStream_t s) {
     return launch_status(2);
 }
 
+// Whether a row at `a` and one at `b` (of `width` bytes, strides in bytes, a stride at least the width) have a byte in common.
+static bool rows_meet(uintptr_t a, __int128 a_stride, uintptr_t b, __int128 b_stride, __int128 width, __int128 rows) {
+    const __int128 apart = (__int128)b - (__int128)a;
+    if (apart >= (rows - 1) * a_stride + width || -apart >= (rows - 1) * b_stride + width) return false;
+    if (a_stride == b_stride) {                                 // row i + k of a lies `rest` before row i of b, row i + k + 1 so much behind that
+        const __int128 k = apart >= 0 ? apart / a_stride : -((-apart + a_stride - 1) / a_stride), rest = apart - k * a_stride;
+        auto there = [&](__int128 d) { return d < rows && -d < rows; };
+        return (there(k) && rest < width) || (there(k + 1) && a_stride - rest < width);
+    }
+    for (__int128 i = 0, j = 0; i < rows && j < rows;) {
+        const __int128 d = apart + j * b_stride - i * a_stride;
+        if (d < width && -d < width) return true;
+        if (d > 0) ++i; else ++j;
+    }
+    return false;
+}
+
 }  // namespace yb
 
 using namespace yb;
@@ -361,6 +378,9 @@ extern "C" int yvex_b200_logits_edit(const yvex_b200_logits_policy *p, const yve
     if (d->drafted && (!d->offsets || !d->row_request || (d->tree && !d->ancestors))) return ERR_INVALID_ARG;
     const uintptr_t size = qtype == Q_F32 ? 4 : 2;
     if (((uintptr_t)logits | (uintptr_t)out) % size || (uintptr_t)grammar % 4) return ERR_INVALID_ARG;
+    if ((logits != out || (logits_stride != out_stride && d->rows > 1)) &&
+        rows_meet((uintptr_t)logits, (__int128)logits_stride * size, (uintptr_t)out, (__int128)out_stride * size, (__int128)p->vocabulary * size, d->rows))
+        return ERR_INVALID_ARG;
     LogitsParams a{*p, *d, logits, logits_stride, grammar, grammar_stride, out, out_stride, 0, 0, status};
     cudaStream_t s = as_stream(stream);
     return qtype == Q_F32 ? launch_logits<float>(a, s) : qtype == Q_BF16 ? launch_logits<__nv_bfloat16>(a, s) : launch_logits<__half>(a, s);
