@@ -81,3 +81,42 @@ def test_logits_and_out_that_overlap_without_being_the_same_rows_are_refused(L):
             (4, P, 1 << 40, P + (3 << 42) + 3996, 1 << 40, 0), (9, P, 1000, P + 4 * 8999, 5000, 0)):
         assert overlap(L, rows, start, stride, out, out_stride, qtype) == -10, (rows, start - P, stride, out - P, out_stride, qtype)
     assert L.lib.yvex_b200_launch_count() == before
+
+
+def test_descriptions_of_another_device_are_refused(front, monkeypatch):
+    """A cache, a step, a policy, drafts or a status made on one device and used while another one is current."""
+    import torch
+
+    class Far(torch.Tensor):                                     # says that it lies on device 3
+        def get_device(self):
+            return 3
+
+    far = lambda t: t.as_subclass(Far)  # noqa: E731
+    k, q, ws = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16), torch.zeros((7, 8, 64), dtype=torch.bfloat16), torch.zeros(64, dtype=torch.uint8)
+    rows, slots, x = torch.zeros((7, 2, 2, 64)), torch.zeros(7, dtype=torch.int64), torch.zeros((3, 100))
+    made = {}
+    for device, on in ((-1, lambda t: t), (3, far)):
+        monkeypatch.setattr(front, "_device", lambda device=device: device)
+        i64 = lambda n: on(torch.zeros(n, dtype=torch.int64))  # noqa: E731
+        made[device] = dict(cache=front.kv_cache_of(on(k), on(k)), geometry=front.kv_geometry_of(4, 16), status=N(word=on(i32(1))),
+                            step=front.kv_step_of(on(i32(3)), on(i32(3)), on(i32(3, 5)), 7, 3, 50, offsets=on(i32(4)), slots=i64(7), positions=on(i32(7)), row_request=on(i32(7))),
+                            policy=front.logits_policy_of(100, on(i32(5)), on(i32(4))), drafts=front.logits_drafts_of(row_request=on(i32(3))))
+    monkeypatch.setattr(front, "_device", lambda: -1)
+    calls = dict(plan=(lambda d: front.kv_plan(d["cache"], d["step"], i32(3), d["status"], i32(1)), ("step", "status")),
+                 append=(lambda d: front.kv_append(d["cache"], slots, rows[:, 0], rows[:, 1], d["status"]), ("cache", "status")),
+                 space=(lambda d: front.attention_paged(d["cache"], d["step"], q, 0.1, d["status"], workspace=ws), ("cache", "step", "status")),
+                 edit=(lambda d: front.logits_edit(d["policy"], d["drafts"], x, d["status"]), ("policy", "drafts", "status")))
+    for name, (call, parts) in calls.items():
+        call(made[-1])
+        for part in parts:
+            with pytest.raises(front.YvexError):
+                call(dict(made[-1], **{part: made[3][part]}))
+    # a plan reads no more of a cache than its sizes, and descriptions without arrays belong to no device
+    for part in ("geometry", "cache"):
+        front.kv_plan(made[3][part], made[-1]["step"], i32(3), status(), i32(1))
+    monkeypatch.setattr(front, "_device", lambda: 3)
+    bare = front.logits_policy_of(100, requests=3), front.logits_drafts_of(rows=3)
+    monkeypatch.setattr(front, "_device", lambda: -1)
+    front.logits_edit(*bare, x, status())
+    with pytest.raises(front.YvexError):
+        front.attention_paged_workspace(made[3]["cache"], made[-1]["step"], 8)

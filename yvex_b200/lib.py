@@ -555,6 +555,17 @@ def _on(dev):
     return raw(dev) if raw else torch.cuda.current_stream(dev).cuda_stream
 
 
+def _here(dev, where, status, *described):
+    """Checks that a status word and descriptions that name arrays are of the current device; the word's address."""
+    for d in described:
+        if d.device is not None and d.device != dev:
+            raise YvexError(INVALID_ARG, where)
+    word = status.word
+    if word.get_device() != dev:
+        raise YvexError(INVALID_ARG, where)
+    return word.data_ptr()
+
+
 def _array(t, dtype, numel, where, dev):
     """Address of a packed array of the given type on device `dev` with at least `numel` elements (None: whatever it has); None for None."""
     if t is None:
@@ -584,7 +595,7 @@ def kv_cache_of(k, v):
           "kv_cache_of")
     pages, heads, page_size, dim = k.shape
     c = KvCache(_qtype_of(k, "kv_cache_of"), pages, page_size, heads, dim, _p(k), _p(v))
-    c._keep, c.dtype, c.row = (k, v), k.dtype, (heads, dim)
+    c._keep, c.dtype, c.row, c.device = (k, v), k.dtype, (heads, dim), dev
     return c
 
 
@@ -606,7 +617,7 @@ def kv_step_of(cached, fresh, block_table, tokens, longest_fresh, longest, paren
     s = KvStep(requests, tokens, block_table.shape[1], longest_fresh, longest, int(tree), at(cached, i32, requests), at(fresh, i32, requests),
                at(parents, i32, tokens), at(block_table, i32, None), at(offsets, i32, requests + 1), at(slots, i64, tokens),
                at(positions, i32, tokens), at(row_request, i32, tokens), at(ancestors, i64, tokens))
-    s._keep, s.rows = (cached, fresh, parents, block_table), tokens
+    s._keep, s.rows, s.device = (cached, fresh, parents, block_table), tokens, dev
     s.offsets_tensor, s.slots_tensor, s.positions_tensor, s.row_request_tensor, s.ancestors_tensor = offsets, slots, positions, row_request, ancestors
     return s
 
@@ -618,7 +629,7 @@ def kv_plan(cache, step, free_pages, status, pages_used=None):
     if pages_used is None:
         pages_used = torch.empty(1, dtype=torch.int32, device=free_pages.device)
     _check(lib.yvex_b200_kv_plan(cache, step, _array(free_pages, torch.int32, None, "kv_plan", dev), free_pages.numel(),
-                                 _array(pages_used, torch.int32, 1, "kv_plan", dev), status.word.data_ptr(), _on(dev)), "kv_plan")
+                                 _array(pages_used, torch.int32, 1, "kv_plan", dev), _here(dev, "kv_plan", status, step), _on(dev)), "kv_plan")
     step.used_tensor = pages_used
     return pages_used
 
@@ -630,12 +641,13 @@ def kv_append(cache, slots, k, v, status):
     tokens, shape = slots.numel(), k.shape
     _need(shape == v.shape and len(shape) == 3 and shape[0] == tokens and shape[1:] == cache.row and k.dtype == v.dtype and k.get_device() == v.get_device() == dev, w)
     _check(lib.yvex_b200_kv_append(cache, _array(slots, torch.int64, None, w, dev), tokens, _qtype_of(k, w), k.data_ptr(), _row_stride(k, w), v.data_ptr(),
-                                   _row_stride(v, w), status.word.data_ptr(), _on(dev)), w)
+                                   _row_stride(v, w), _here(dev, w, status, cache), _on(dev)), w)
 
 
 def attention_paged_workspace(cache, step, q_heads):
     """Scratch for attention_paged calls of this cache and step sizes."""
-    torch = _torch()
+    torch, dev = _torch(), _device()
+    _need(cache.device == dev and step.device == dev, "attention_paged_workspace")
     n = int(lib.yvex_b200_attention_paged_workspace_bytes(cache, step, q_heads))
     _need(n > 0, "attention_paged_workspace")
     return torch.empty(n, dtype=torch.uint8, device="cuda")
@@ -646,7 +658,7 @@ def attention_paged(cache, step, q, scale, status, workspace=None, out=None):
     torch, dev, w = _torch(), _device(), "attention_paged"
     shape, dtype = q.shape, q.dtype
     _need(len(shape) == 3 and shape[0] == step.rows and shape[2] == cache.row[1] and dtype == cache.dtype and q.get_device() == dev, w)
-    heads = shape[1]
+    heads, word = shape[1], _here(dev, w, status, cache, step)
     if workspace is None:
         workspace = attention_paged_workspace(cache, step, heads)
     else:
@@ -654,7 +666,7 @@ def attention_paged(cache, step, q, scale, status, workspace=None, out=None):
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=q.device)
     _check(lib.yvex_b200_attention_paged(cache, step, q.data_ptr(), _row_stride(q, w), heads, scale, _array(out, dtype, q.numel(), w, dev),
-                                         _array(workspace, torch.uint8, None, w, dev), workspace.numel(), status.word.data_ptr(), _on(dev)), w)
+                                         _array(workspace, torch.uint8, None, w, dev), workspace.numel(), word, _on(dev)), w)
     return out
 
 
@@ -674,6 +686,7 @@ def logits_policy_of(vocabulary, history=None, history_offsets=None, prompt_leng
                      at(prompt_lengths, i32, requests), at(repetition, f32, requests), at(presence, f32, requests), at(frequency, f32, requests),
                      at(bias_tokens, i32, None), at(bias_values, f32, count(bias_tokens)), at(bias_offsets, i32, requests + 1))
     p._keep = (history, history_offsets, prompt_lengths, repetition, presence, frequency, bias_tokens, bias_values, bias_offsets)
+    p.device = None if all(t is None for t in p._keep) else dev
     return p
 
 
@@ -686,6 +699,7 @@ def logits_drafts_of(drafted=None, row_request=None, offsets=None, ancestors=Non
     d = LogitsDrafts(rows, int(tree), _array(drafted, torch.int32, rows, w, dev), _array(row_request, torch.int32, rows, w, dev),
                      _array(offsets, torch.int32, None, w, dev), _array(ancestors, torch.int64, rows, w, dev))
     d._keep, d.requests = (drafted, row_request, offsets, ancestors), None if offsets is None else offsets.numel() - 1
+    d.device = None if all(t is None for t in d._keep) else dev
     return d
 
 
@@ -703,7 +717,7 @@ def logits_edit(policy, drafts, logits, status, grammar=None, out=None):
         _need(grammar.dim() == 2 and grammar.shape[0] >= rows and grammar.dtype == torch.int32 and grammar.stride(1) == 1 and grammar.get_device() == dev, w)
         address, words = grammar.data_ptr(), _pitch(grammar)
     _check(lib.yvex_b200_logits_edit(policy, drafts, _qtype_of(logits, w), logits.data_ptr(), _pitch(logits), address, words, out.data_ptr(), _pitch(out),
-                                     status.word.data_ptr(), _on(dev)), w)
+                                     _here(dev, w, status, policy, drafts), _on(dev)), w)
     return out
 
 
