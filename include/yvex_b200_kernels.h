@@ -496,7 +496,7 @@ int yvex_b200_kv_append(const yvex_b200_kv_cache *cache, const int64_t *slots, u
 /*
  * Attention of the fresh tokens over the pages, their own rows among them (append comes first): q [tokens] rows of
  * [q_heads][head_dim] in the cache's type (q_stride: elements between rows, 16-byte aligned), out packed alike in the
- * cache's type, f32 scores, softmax and sums. Query heads share kv heads in groups of q_heads / kv_heads. A row that
+ * cache's type, f32 scores, softmax and sums (numbers under 2^-126 may count as zero there). scale is at least 2^-126, and finite times log2 e. Query heads share kv heads in groups of q_heads / kv_heads. A row that
  * sees no key (an empty mask over an empty cache) is zero; padding rows of out are left as they were. Keys that a row does
  * not see have no influence on it, whatever is stored there. Of the step's arrays cached, block_table, offsets and ancestors
  * (trees) are read. Status 1: an output that is not finite; 2: lengths above their bounds, offsets that are not those of a

@@ -183,3 +183,18 @@ def test_attention_one_key_far_above_the_others(L, above, group, dtype):  # noqa
     L.attention_paged(cache, s.step, q, 1.0, s.status, out=out)
     assert s.status.read() == 0
     check_attention(s, out, q, k, v, 1.0)
+
+
+@pytest.mark.parametrize("fresh", [1, 40])
+@pytest.mark.parametrize("scale", [1.1755e-38, 1e-30, 2.358e38])
+def test_attention_smallest_and_largest_scales(L, scale, fresh):  # noqa: F811
+    """At both ends of what is taken: every key has the same weight (with the largest scale, for queries of zero)."""
+    import torch
+    s = Step(L, [500, 3], [fresh, 2], 32)
+    _, q, k, v, cache = attend(L, s, 2, 4, 128, "bfloat16")
+    if scale > 1:
+        q.zero_()
+    out = torch.full_like(q, 7.0)
+    L.attention_paged(cache, s.step, q, scale, s.status, out=out)
+    assert s.status.read() == 0
+    check_attention(s, out, q, k, v, scale)

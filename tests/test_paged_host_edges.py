@@ -120,3 +120,13 @@ def test_descriptions_of_another_device_are_refused(front, monkeypatch):
     front.logits_edit(*bare, x, status())
     with pytest.raises(front.YvexError):
         front.attention_paged_workspace(made[3]["cache"], made[-1]["step"], 8)
+
+
+def test_scales_that_f32_cannot_carry_are_refused(L):
+    """A subnormal scale is zero where the exponentials are computed (and zero times the -inf of an unseen key is NaN), and one near the
+    largest number is infinite once it is in powers of two."""
+    P, before = 0x10000, L.lib.yvex_b200_launch_count()
+    cache, step = L.KvCache(30, 100, 16, 2, 128, P, P), L.KvStep(3, 12, 5, 4, 80, 0, P, P, P, P, P, P, P, P, P)
+    for scale in (1e-40, 1.1e-38, 1e-45, 2.4e38, 3.4e38):
+        assert L.lib.yvex_b200_attention_paged(cache, step, P, 1024, 8, scale, P, P, 1 << 40, P, None) == -10
+    assert L.lib.yvex_b200_launch_count() == before

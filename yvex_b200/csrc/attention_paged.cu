@@ -11,6 +11,7 @@
 // 64 sessions of 100 to 32768 keys (3.46 GB): 558 us, 6.2 TB/s, 94 % of the copy bandwidth; equal shares of blocks instead of a fixed number of
 // slices per session are what holds that for ragged lengths. One session of 1500 keys: 12 us for the two kernels, all latency.
 #include <cuda_bf16.h>
+#include <float.h>
 
 #include <initializer_list>
 
@@ -342,7 +343,7 @@ extern "C" int yvex_b200_attention_paged(const yvex_b200_kv_cache *c, const yvex
     const int rc = paged_refusal(c, t, q_heads);
     if (rc != OK) return rc;
     if (!q || !out || !status || !t->cached || !t->offsets || !t->block_table || (t->tree && !t->ancestors)) return ERR_INVALID_ARG;
-    if (!isfinite(scale) || scale <= 0.0f) return ERR_INVALID_ARG;
+    if (!(scale >= FLT_MIN) || !isfinite(scale * 1.4426950408889634f)) return ERR_INVALID_ARG;
     if (q_stride < q_heads * c->head_dim) return ERR_BOUNDS;
     if (((uintptr_t)q | (uintptr_t)out) & 15u || q_stride % 8) return ERR_INVALID_ARG;
     const PagedShape s = paged_shape(c, t, q_heads);
