@@ -100,6 +100,71 @@ def test_logits_beside_out_in_one_buffer(L):  # noqa: F811
         assert kind == "in_place" or torch.equal(rows, x), kind
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_logits_more_rows_than_a_grid_has(L, dtype):  # noqa: F811
+    """70 000 rows of a small vocabulary, of 35 000 requests with a history of two words each; every seventh row is padding."""
+    import torch
+    rows, R, V = 70000, 35000, 37
+    rng = np.random.default_rng(3)
+    x = torch.tensor(rng.normal(0, 3, (rows, V)).astype(np.float32), device="cuda").to(getattr(torch, dtype))
+    request = np.arange(rows) // 2
+    request[::7] = -1
+    history, frequency = rng.integers(0, V, (R, 2)).astype(np.int32), rng.uniform(0, 0.5, R).astype(np.float32)
+    policy = L.logits_policy_of(V, ints(history.reshape(-1)), ints(np.arange(R + 1) * 2), frequency=ints(frequency, torch.float32))
+    st, out = L.Status(), torch.full_like(x, 7.0)
+    before = out.clone()
+    L.logits_edit(policy, L.logits_drafts_of(row_request=ints(request)), x, st, out=out)
+    assert st.read() == 0
+    want, count = x.double().cpu().numpy(), np.zeros((R, V))
+    np.add.at(count, (np.repeat(np.arange(R), 2), history.reshape(-1)), 1)
+    want -= frequency[request][:, None].astype(np.float64) * count[request]
+    check_edit(out, want, request, before)
+
+
+def test_logits_captured_and_replayed_with_other_words(L):  # noqa: F811
+    """Two graphs on two streams, replayed while histories, offsets, paths, masks and rows change; the results are those of calls one at a time."""
+    import torch
+    V, R, rows, most = 20000, 3, 9, 4000
+    made = []
+    for g in range(2):
+        rng = np.random.default_rng(g)
+        t = dict(history=ints([0] * most), offsets=ints([0] * (R + 1)), penalty=ints([1.0] * R, torch.float32), drafted=ints([0] * rows), request=ints([0] * rows),
+                 begin=ints([0] * (R + 1)), ancestors=ints([0] * rows, torch.int64), grammar=ints([[0] * 625] * rows), x=torch.zeros((rows, V), device="cuda"))
+        policy = L.logits_policy_of(V, t["history"], t["offsets"], None, t["penalty"], t["penalty"], t["penalty"])
+        drafts, st, out, stream = L.logits_drafts_of(t["drafted"], t["request"], t["begin"], t["ancestors"], tree=True), L.Status(), torch.zeros((rows, V), device="cuda"), torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            L.logits_edit(policy, drafts, t["x"], st, grammar=t["grammar"], out=out)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                L.logits_edit(policy, drafts, t["x"], st, grammar=t["grammar"], out=out)
+        made.append((rng, t, policy, drafts, st, out, stream, graph))
+    torch.cuda.synchronize()
+    for st in (m[4] for m in made):
+        st.reset()                                               # (the first call's rows lay outside their request)
+    torch.cuda.synchronize()
+    for fresh in ([4, 0, 5], [1, 1, 1], [0, 0, 9]):
+        for rng, t, policy, drafts, st, out, stream, graph in made:
+            with torch.cuda.stream(stream):
+                n, history = sum(fresh), [int(h) for h in rng.integers(0, most // R, R)]
+                at = np.concatenate([[0], np.cumsum(history)])
+                new = dict(history=rng.integers(0, V, most), offsets=at, drafted=rng.integers(0, V, rows), begin=np.concatenate([[0], np.cumsum(fresh)]),
+                           request=sum(([r] * f for r, f in enumerate(fresh)), []) + [-1] * (rows - n),
+                           ancestors=[(1 << i) | 1 for f in fresh for i in range(f)] + [0] * (rows - n), grammar=rng.integers(-2 ** 31, 2 ** 31, (rows, 625)))
+                for name, value in new.items():
+                    t[name].copy_(ints(np.asarray(value).tolist(), t[name].dtype))
+                t["penalty"].uniform_(0.5, 1.5)
+                t["x"].normal_()
+                out.fill_(7.0)
+                graph.replay()
+        torch.cuda.synchronize()
+        for rng, t, policy, drafts, st, out, stream, graph in made:
+            alone = torch.full_like(out, 7.0)
+            assert st.read() == 0
+            L.logits_edit(policy, drafts, t["x"], st, grammar=t["grammar"], out=alone)
+            assert st.read() == 0 and torch.equal(out, alone) and bool((out[sum(fresh):] == 7.0).all())
+
+
 # ---- plan: requests whose lengths are bad -----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("tree", [None, "random"])
@@ -198,3 +263,42 @@ def test_attention_smallest_and_largest_scales(L, scale, fresh):  # noqa: F811
     L.attention_paged(cache, s.step, q, scale, s.status, out=out)
     assert s.status.read() == 0
     check_attention(s, out, q, k, v, scale)
+
+
+# ---- attention: more requests than a CTA counts at a time -------------------------------------------------------------
+
+@pytest.mark.parametrize("requests,most,tree", [(127, 2, None), (128, 1, None), (129, 2, None), (300, 1, None), (1100, 2, None), (390, 20, None), (390, 40, "random"), (800, 20, "star"), (33, 140, None),
+                                                (49, 140, None)])
+@pytest.mark.parametrize("dtype,dim,group", [("bfloat16", 128, 2), ("float16", 256, 4), ("float16", 64, 3)])
+def test_attention_of_more_requests_than_a_cta_has_threads(L, requests, most, tree, dtype, dim, group):  # noqa: F811
+    """Lengths counted in several rounds, with bad ones among them (whose rows stay as they were) and long runs without fresh tokens."""
+    import torch
+    rng = np.random.default_rng(requests + most)
+    fresh = (rng.integers(1, min(most, 6) + 1, requests) * (rng.random(requests) < 0.7)).tolist()
+    for r in range(requests // 3, requests // 3 + requests // 5):
+        fresh[r] = 0
+    fresh[-1] = most
+    cached = (300 * rng.random(requests) ** 3).astype(int).tolist()
+    s = Step(L, cached, fresh, 16, seed=most, tree=tree)
+    out, q, k, v, cache = attend(L, s, 2, group, dim, dtype, most)
+    assert s.status.read() == 0
+    check_attention(s, out, q, k, v)
+    # a request whose cached tokens are more than there can be, in the middle
+    bad = requests // 2 + requests // 8
+    s.cached_dev[bad] = 1 << 20
+    got = torch.full_like(out, 7.0)
+    L.attention_paged(cache, s.step, q, dim ** -0.5, s.status, out=got)
+    assert s.status.read() == 2
+    b, e = s.want["offsets"][bad], s.want["offsets"][bad + 1]
+    assert bool((got[b:e] == 7.0).all())
+    got[b:e] = out[b:e]                                          # the others: as before, but for shares that are cut elsewhere
+    check_attention(s, got, q, k, v)
+
+
+@pytest.mark.parametrize("most", [1, 40])
+def test_attention_of_a_step_without_fresh_tokens(L, most):  # noqa: F811
+    """A captured step whose requests all wait: nothing is written and nothing reported."""
+    s = Step(L, [30, 0, 100], [0, 0, 0], 16, extra_tokens=3)
+    s.step.longest_fresh = most
+    out, q, k, v, _ = attend(L, s, 2, 4, 128, "bfloat16")
+    assert s.status.read() == 0 and bool((out == 7.0).all())
