@@ -2,8 +2,10 @@
 //
 // Two kernels. The first streams the rows through with nothing but the grammar's mask: bound by HBM (8 bytes a word for f32 rows). The
 // second edits the words that occur in a request's history, on a row's path or among its biases, a few in a hundred, in place: a CTA
-// takes several rows of a request, counts its words in a hash table in shared memory (key, one 32-bit counter: bit 31 occurs in the
-// prompt, the rest how often it was generated, and, where there are biases, the last entry of the word), and then visits the table's words for every row. The table is built while the
+// takes several rows of a request, counts its words in a hash table in shared memory (key, and one 32-bit counter: bit 31 occurs in the
+// prompt, the rest how often it was generated), and then visits the table's words for every row. Biased words enter the table first, so that they are
+// the first of its list and their last entries an array beside it (a place for them in every slot, 229 KB of shared memory in place of 160, took 24 us
+// more at 419 rows). The table is built while the
 // stream runs. Counters are integers, so the order of the atomics does not show. Requests with more words than the table holds are done in
 // parts of the words, halved until they fit. (One kernel with counters for a share of the vocabulary and the edits in the stream took 204 us for
 // 419 rows of 129280 words, with the edits behind the stream 175: nearly every warp meets a counted word among its 128, and every share
@@ -16,7 +18,7 @@ namespace yb {
 constexpr int kStreamThreads = 256, kStreamLoads = 4, kStreamCtas = 4;      // of the stream: loads of 16 bytes, CTAs an SM
 constexpr int kEditThreads = 1024, kEditsAhead = 4;       // of the edits: words a thread has on their way
 constexpr uint32_t kSeen = 1u << 31, kCount = kSeen - 1u;
-constexpr uint32_t kLeastTable = 1024, kMostTable = 16384;
+constexpr uint32_t kLeastTable = 1024, kMostTable = 16384, kMostBiased = 8192;      // slots; biased words of a table
 
 struct LogitsParams {
     yvex_b200_logits_policy p;
@@ -27,7 +29,7 @@ struct LogitsParams {
     uint64_t grammar_stride;
     void *out;
     uint64_t out_stride;
-    uint32_t table_log2, rows_per_cta;
+    uint32_t table_log2, biased, rows_per_cta;         // biased: places for biased words
     int *status;
 };
 
@@ -149,14 +151,13 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamCtas) logits_stream_ker
 // blockIdx.x: the rows, blockIdx.y of gridDim.y (a power of two): the words.
 template <class T>
 __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsParams a) {
-    extern __shared__ __align__(16) uint32_t keys[];    // words (~0: none), their counters, the list of those in use, the last bias entries (-1: none)
+    extern __shared__ __align__(16) uint32_t keys[];    // words (~0: none), their counters, the list of those in use, the last bias entries of the list's first
     __shared__ int list_count;
     const int tid = threadIdx.x;
     const uint32_t slots = 1u << a.table_log2, limit = slots / 4 * 3, vocabulary = (uint32_t)a.p.vocabulary;
     uint32_t *counters = keys + slots;
     uint16_t *list = reinterpret_cast<uint16_t *>(counters + slots);
-    int *last_bias = reinterpret_cast<int *>(list + slots);
-    const bool biased = a.p.bias_tokens != nullptr;
+    int *last_bias = reinterpret_cast<int *>(list + limit);
     const uint64_t first_row = (uint64_t)blockIdx.x * a.rows_per_cta, last_row = min(a.d.rows, first_row + a.rows_per_cta);
     bool bad_arg = false, bad_num = false, waited = false;
     uint32_t parts = gridDim.y, part = blockIdx.y;      // words of that part are in the table
@@ -166,8 +167,9 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
     // second hash say which, so that neither a step between the words (their low bits alone make the low bits of the first) nor
     // the place in the table, which the first one's high bits give, tells the part.
     auto part_of = [&](uint32_t h) { return __umulhi(hash(h ^ (h >> 15)), parts); };
-    // The slot of word w, which is entered if it is not there; -1 for padding, words of other parts, and when the table is full.
-    auto slot_of = [&](int32_t w) -> int {
+    // The slot of word w, which is entered if it is not there (`numbered`: with its place in the list as its counter); -1 for padding, words of
+    // other parts, and when the table is full.
+    auto slot_of = [&](int32_t w, bool numbered) -> int {
         if (w < 0) return -1;
         if ((uint32_t)w >= vocabulary) { bad_arg = true; return -1; }
         const uint32_t h = hash((uint32_t)w);
@@ -183,7 +185,8 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
                     int n = 0;
                     if (lane == leader) n = atomicAdd(&list_count, __popc(m));
                     n = __shfl_sync(m, n, (int)leader) + __popc(m & ((1u << lane) - 1u));
-                    if (n < (int)slots) list[n] = (uint16_t)s;
+                    if (n < (int)limit) list[n] = (uint16_t)s;
+                    if (numbered) counters[s] = (uint32_t)n;
                     return (int)s;
                 }
             }
@@ -221,6 +224,7 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
         }
         const int64_t paths_end = a.d.tree ? min(end, begin + YVEX_B200_TREE_NODES) : min(end, (int64_t)stop);      // words that a path may have
 
+        const int32_t first_biased = bias_from + tid < bias_to ? a.p.bias_tokens[bias_from + tid] : -1;      // (on its way while the table is cleared)
         parts = gridDim.y;
         part = blockIdx.y;
         for (;;) {
@@ -228,35 +232,47 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
             __syncthreads();
             for (uint32_t i = tid; i < slots / 2; i += kEditThreads)
                 reinterpret_cast<uint4 *>(keys)[i] = i < slots / 4 ? make_uint4(~0u, ~0u, ~0u, ~0u) : make_uint4(0, 0, 0, 0);
-            for (uint32_t i = tid; biased && i < slots / 4; i += kEditThreads) reinterpret_cast<int4 *>(last_bias)[i] = make_int4(-1, -1, -1, -1);
+            for (uint32_t i = tid; i < a.biased; i += kEditThreads) last_bias[i] = -1;
             if (tid == 0) list_count = 0;
             __syncthreads();
+            int biased = 0;                             // the list's words up to here have biases
+            if (bias_to > bias_from) {
+                const int first = slot_of(first_biased, true);
+                for (int64_t t = bias_from + tid + kEditThreads; t < bias_to; t += kEditThreads) slot_of(a.p.bias_tokens[t], true);
+                __syncthreads();
+                biased = list_count;
+                if (biased > (int)min(limit, a.biased)) { parts *= 2u; part *= 2u; continue; }      // too many words: half of them first
+                if (first >= 0) atomicMax(&last_bias[counters[first]], (int)(bias_from + tid));
+                for (int64_t t = bias_from + tid + kEditThreads; t < bias_to; t += kEditThreads) {
+                    const int s = slot_of(a.p.bias_tokens[t], true);      // (every word is there now)
+                    if (s >= 0) atomicMax(&last_bias[counters[s]], (int)t);
+                }
+                __syncthreads();
+                for (int i = tid; i < biased; i += kEditThreads) counters[list[i]] = 0;
+                __syncthreads();
+            }
             for (int64_t t0 = from + tid; t0 < to; t0 += 4 * kEditThreads) {
                 int32_t w[4];                           // (four words on their way at a time)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) w[q] = t0 + q * kEditThreads < to ? a.p.history[t0 + q * kEditThreads] : -1;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int s = slot_of(w[q]);
+                    const int s = slot_of(w[q], false);
                     if (s < 0) continue;
                     if (t0 + q * kEditThreads >= prompt) atomicAdd(&counters[s], 1u);
                     else if (!(counters[s] & kSeen)) atomicOr(&counters[s], kSeen);
                 }
             }
-            for (int64_t t = bias_from + tid; t < bias_to; t += kEditThreads) {
-                const int s = slot_of(a.p.bias_tokens[t]);
-                if (s >= 0) atomicMax(&last_bias[s], (int)t);
-            }
             // drafted words have their slots before the first row; a tree's nodes keep a thread each
             int node = -1;
             for (int64_t t = begin + tid; t < paths_end; t += kEditThreads) {
-                const int s = slot_of(a.d.drafted[t]);
+                const int s = slot_of(a.d.drafted[t], false);
                 if (a.d.tree) node = s;
                 else if (t < (int64_t)row && s >= 0) atomicAdd(&counters[s], 1u);      // (the chain before the first row)
             }
             __syncthreads();
             const int n = list_count;
-            if (n > (int)limit) { parts *= 2u; part *= 2u; continue; }      // too many words: half of them first
+            if (n > (int)limit) { parts *= 2u; part *= 2u; continue; }
 
             if (!waited) { pdl_wait(); waited = true; }                     // the stream has written the rows
             for (uint64_t t = row; t < stop; ++t) {
@@ -266,7 +282,7 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
                 bool on = false;                        // this thread's node is on the path
                 if (a.d.drafted && end > begin) {
                     if (a.d.tree) on = node >= 0 && (a.d.ancestors[t] >> tid) & 1ull;
-                    else if (tid == 0) node = slot_of(a.d.drafted[t]), on = node >= 0;
+                    else if (tid == 0) node = slot_of(a.d.drafted[t], false), on = node >= 0;
                     if (on) atomicAdd(&counters[node], 1u);
                     __syncthreads();
                 }
@@ -277,7 +293,7 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
                     for (int q = 0; q < kEditsAhead; ++q) {     // (in place, the stream has left the words as they were, or -inf where the grammar forbids them)
                         const int i = i0 + q * kEditThreads;
                         slot[q] = i < n ? list[i] : -1;
-                        if (slot[q] >= 0 && !counters[slot[q]] && !(biased && last_bias[slot[q]] >= 0)) slot[q] = -1;
+                        if (slot[q] >= 0 && i >= biased && !counters[slot[q]]) slot[q] = -1;
                         if (slot[q] >= 0) x[q] = LogitsVec<T>::get(in + keys[slot[q]]);
                     }
 #pragma unroll
@@ -290,8 +306,7 @@ __global__ void __launch_bounds__(kEditThreads) logits_edit_kernel(const LogitsP
                             y = y > 0.0f ? y / rep : y * rep;
                             if (times) y -= frequency * (float)times + presence;
                         }
-                        const int last = biased ? last_bias[s] : -1;      // the last entry of a word counts
-                        if (last >= 0) y += a.p.bias_values[last];
+                        if (const int i = i0 + q * kEditThreads; i < biased) y += a.p.bias_values[last_bias[i]];      // the last entry of a word counts
                         if (!allows(allowed, word)) y = -INFINITY;
                         bad_num |= y != y;
                         LogitsVec<T>::put(out + word, y);
@@ -330,16 +345,16 @@ template <class T> static int launch_logits(LogitsParams &a, cudaStream_t s) {
     uint32_t slots = kLeastTable;
     a.table_log2 = 10;
     while (slots < 2 * words && slots < kMostTable) { slots *= 2; ++a.table_log2; }
-    constexpr uint64_t per_word = 2 * sizeof(uint32_t) + sizeof(uint16_t);
-    const uint64_t per_slot = per_word + (a.p.bias_tokens ? sizeof(int) : 0);
-    const int rc = optin.ensure(logits_edit_kernel<T>, (int)(kMostTable * (per_word + sizeof(int))));
+    constexpr uint64_t four_slots = 4 * 2 * sizeof(uint32_t) + 3 * sizeof(uint16_t);
+    a.biased = a.p.bias_tokens ? (uint32_t)(a.p.bias_entries < kMostBiased ? a.p.bias_entries : kMostBiased) : 0u;
+    const int rc = optin.ensure(logits_edit_kernel<T>, (int)(kMostTable / 4 * four_slots + kMostBiased * sizeof(int)));
     if (rc != OK) return rc;
     uint64_t parts = 1;
     while (a.d.rows * parts * 2 <= kSmCount && parts * 128 < words) parts *= 2;
     const uint64_t ctas = (uint64_t)kSmCount * (slots >= kMostTable ? 1 : 2) / parts;
     a.rows_per_cta = (uint32_t)((a.d.rows + ctas - 1) / ctas);
     const uint64_t chunks = (a.d.rows + a.rows_per_cta - 1) / a.rows_per_cta;
-    if (launch_pdl(logits_edit_kernel<T>, dim3((unsigned)chunks, (unsigned)parts), dim3(kEditThreads), (size_t)(slots * per_slot), s, a) != cudaSuccess) return ERR_BACKEND;
+    if (launch_pdl(logits_edit_kernel<T>, dim3((unsigned)chunks, (unsigned)parts), dim3(kEditThreads), (size_t)(slots / 4 * four_slots + a.biased * sizeof(int)), s, a) != cudaSuccess) return ERR_BACKEND;
     return launch_status(2);
 }
 
@@ -381,7 +396,7 @@ extern "C" int yvex_b200_logits_edit(const yvex_b200_logits_policy *p, const yve
     if ((logits != out || (logits_stride != out_stride && d->rows > 1)) &&
         rows_meet((uintptr_t)logits, (__int128)logits_stride * size, (uintptr_t)out, (__int128)out_stride * size, (__int128)p->vocabulary * size, d->rows))
         return ERR_INVALID_ARG;
-    LogitsParams a{*p, *d, logits, logits_stride, grammar, grammar_stride, out, out_stride, 0, 0, status};
+    LogitsParams a{*p, *d, logits, logits_stride, grammar, grammar_stride, out, out_stride, 0, 0, 0, status};
     cudaStream_t s = as_stream(stream);
     return qtype == Q_F32 ? launch_logits<float>(a, s) : qtype == Q_BF16 ? launch_logits<__nv_bfloat16>(a, s) : launch_logits<__half>(a, s);
 }
