@@ -78,6 +78,32 @@ def test_logits_long_bias_lists(L, rows):  # noqa: F811
     assert begin.elapsed_time(end) < (10.0 if rows == 80 else 2.0), begin.elapsed_time(end)
 
 
+@pytest.mark.parametrize("lists", [[2561, 0, 0], [7000, 3, 500], [8192, 9000], [2560, 2560], [12289, 12289], [0, 20000]])
+def test_logits_bias_lists_of_uneven_lengths(L, lists):  # noqa: F811
+    """As many biased words as there are places for, one more, and many more, beside requests with few or none; histories and paths among them."""
+    import torch
+    V, R = 40000, len(lists)
+    rng = np.random.default_rng(sum(lists))
+    tokens = np.concatenate([rng.permutation(V)[:n] for n in lists]).astype(np.int32)
+    values, off = rng.normal(0, 5, len(tokens)).astype(np.float32), np.concatenate([[0], np.cumsum(lists)])
+    request = np.arange(3 * R) // 3
+    history, drafted = rng.integers(0, V, (R, 900)).astype(np.int32), rng.integers(0, V, 3 * R).astype(np.int32)
+    x = torch.randn((3 * R, V), device="cuda", generator=torch.Generator(device="cuda").manual_seed(R))
+    want = x.double().cpu().numpy()
+    for t, r in enumerate(request):
+        count = np.bincount(np.concatenate([history[r], drafted[3 * r:t + 1]]), minlength=V)
+        want[t] = np.where(count > 0, np.where(want[t] > 0, want[t] / 1.25, want[t] * 1.25), want[t]) - 0.125 * count
+        want[t, tokens[off[r]:off[r + 1]]] += values[off[r]:off[r + 1]]
+    policy = L.logits_policy_of(V, ints(history.reshape(-1)), ints(np.arange(R + 1) * 900), None, ints([1.25] * R, torch.float32), None, ints([0.125] * R, torch.float32),
+                                ints(tokens), ints(values, torch.float32), ints(off))
+    drafts, st = L.logits_drafts_of(ints(drafted), ints(request), ints(np.arange(R + 1) * 3)), L.Status()
+    out = L.logits_edit(policy, drafts, x, st)
+    assert st.read() == 0
+    check_edit(out, want, list(request), out)
+    L.logits_edit(policy, drafts, x, st, out=x)
+    assert st.read() == 0 and torch.equal(x, out)
+
+
 def test_logits_beside_out_in_one_buffer(L):  # noqa: F811
     """Rows of logits and of out that lie among one another without overlapping, with equal strides and different ones, and in place with a stride."""
     import torch

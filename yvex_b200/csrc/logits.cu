@@ -18,7 +18,7 @@ namespace yb {
 constexpr int kStreamThreads = 256, kStreamLoads = 4, kStreamCtas = 4;      // of the stream: loads of 16 bytes, CTAs an SM
 constexpr int kEditThreads = 1024, kEditsAhead = 4;       // of the edits: words a thread has on their way
 constexpr uint32_t kSeen = 1u << 31, kCount = kSeen - 1u;
-constexpr uint32_t kLeastTable = 1024, kMostTable = 16384, kMostBiased = 8192;      // slots; biased words of a table
+constexpr uint32_t kLeastTable = 1024, kMostTable = 16384, kFewBiased = 2560, kMostBiased = 8192;      // slots; biased words of a table
 
 struct LogitsParams {
     yvex_b200_logits_policy p;
@@ -346,7 +346,11 @@ template <class T> static int launch_logits(LogitsParams &a, cudaStream_t s) {
     a.table_log2 = 10;
     while (slots < 2 * words && slots < kMostTable) { slots *= 2; ++a.table_log2; }
     constexpr uint64_t four_slots = 4 * 2 * sizeof(uint32_t) + 3 * sizeof(uint16_t);
-    a.biased = a.p.bias_tokens ? (uint32_t)(a.p.bias_entries < kMostBiased ? a.p.bias_entries : kMostBiased) : 0u;
+    // Places for 2560 biased words leave the shared memory at 164 KB and the rest as cache; more are taken where a request has more on average, whose
+    // words would else be counted in more parts (416 rows of 16 requests, us with 2560 and with 8192: 300 biases each 142 and 145, 1000 163
+    // and 167, 2000 187 and 192, 4000 266 and 237, 10000 582 and 468).
+    const uint64_t places = a.p.bias_entries > kFewBiased * a.p.requests ? kMostBiased : kFewBiased;
+    a.biased = a.p.bias_tokens ? (uint32_t)(a.p.bias_entries < places ? a.p.bias_entries : places) : 0u;
     const int rc = optin.ensure(logits_edit_kernel<T>, (int)(kMostTable / 4 * four_slots + kMostBiased * sizeof(int)));
     if (rc != OK) return rc;
     uint64_t parts = 1;
