@@ -328,3 +328,37 @@ def test_attention_of_a_step_without_fresh_tokens(L, most):  # noqa: F811
     s.step.longest_fresh = most
     out, q, k, v, _ = attend(L, s, 2, 4, 128, "bfloat16")
     assert s.status.read() == 0 and bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("fresh,tree", [(1, None), (4, None), (40, "random")])
+def test_attention_of_pages_that_the_kernel_before_has_written_again(L, fresh, tree):  # noqa: F811
+    """Pages, slots and queries are written anew before every attention, with nothing waited for between them: no call sees what an earlier
+    one has read from the same places."""
+    import torch
+    def go(wait):
+        s = Step(L, [500, 200], [fresh, fresh], 16, tree=tree)
+        gen = torch.Generator(device="cuda").manual_seed(11)
+        k, v = (torch.zeros((s.pages, 2, 16, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        cache, outs = L.kv_cache_of(k, v), []
+        s.plan()
+        tables = [s.table_dev.clone() for _ in range(2)]
+        tables[1][:, :12] = s.table_dev[:, :12].flip(1)          # the same pages in another order
+        every = torch.arange(s.pages * 16, device="cuda")
+        ws, rows = L.attention_paged_workspace(cache, s.step, 8), torch.empty((s.pages * 16, 2, 2, 128), dtype=torch.bfloat16, device="cuda")
+        q = torch.empty((s.tokens, 8, 128), dtype=torch.bfloat16, device="cuda")
+        for i in range(24):
+            rows.normal_(generator=gen)
+            q.normal_(generator=gen)
+            s.table_dev.copy_(tables[i % 2])
+            slots = every.roll(i)
+            L.kv_append(cache, slots, rows[:, 0], rows[:, 1], s.status)
+            for _ in range(2):                                   # (the second call's kernels follow the first's)
+                outs.append(L.attention_paged(cache, s.step, q, 0.1, s.status, workspace=ws))
+            L.kv_append(cache, every, rows[:, 1], rows[:, 0], s.status)
+            outs.append(L.attention_paged(cache, s.step, q, 0.1, s.status, workspace=ws))
+            if wait:
+                torch.cuda.synchronize()
+        assert s.status.read() == 0
+        return outs
+    for a, b in zip(go(False), go(True)):
+        assert torch.equal(a, b) and torch.isfinite(a).all()

@@ -32,9 +32,10 @@ template <class T> __device__ __forceinline__ void mma16816(float (&d)[4], uint3
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// (Not through the read-only path, here and for the tables: the kernel may begin while the one before it still writes what is read after the wait.)
 __device__ __forceinline__ uint4 ldg_once(const uint16_t *p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
 
@@ -71,7 +72,7 @@ __global__ void __launch_bounds__(kRowsThreads, R == 8 && D <= 128 ? 3 : 2) page
             const uint16_t *src = p.q + (uint64_t)(w.q.n.token + token) * p.q_stride + ((uint64_t)w.head * p.group + row % p.group) * D;
 #pragma unroll
             for (int i = 0; i < KL; ++i) {
-                const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src) + c + 4 * i) : make_uint4(0, 0, 0, 0);
+                const uint4 v = live ? reinterpret_cast<const uint4 *>(src)[c + 4 * i] : make_uint4(0, 0, 0, 0);
                 qa[h][i][0] = v.x; qa[h][i][1] = v.y; qa[h][i][2] = v.z; qa[h][i][3] = v.w;
             }
             seen[h] = live ? cached + token + 1 : cached;
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(kRowsThreads, R == 8 && D <= 128 ? 3 : 2) page
                 for (int e = 0; e < 4; ++e) acc[u][j][e] = 0.0f;
 
         auto page_of = [&](int64_t base) -> int32_t {           // the page of the 16 keys from base on; -1 past the end
-            return base < end ? __ldg(table + (uint32_t)(base / 16) / units_per_page) : -1;
+            return base < end ? table[(uint32_t)(base / 16) / units_per_page] : -1;
         };
         int64_t base = (int64_t)w.first * kRowsBlock + 16 * warp;
         int32_t page = page_of(base);

@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                 none = false;
                 const uint32_t key = (w.first + j) * BK + (uint32_t)(lane * box_keys);
                 if (lane >= boxes || j >= w.count || key >= end) return nowhere;
-                const int32_t page = __ldg(table + key / page_size);
+                const int32_t page = table[key / page_size];
                 none = page < 0 || (uint64_t)page >= p.pages;
                 return none ? nowhere : ((uint32_t)page * p.kv_heads + w.head) * page_size + key % page_size;
             };

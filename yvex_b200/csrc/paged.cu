@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanParams 
 
 // ---- append -------------------------------------------------------------------------------------------------------------
 // A copy with one rounding, bound by HBM (16384 tokens x 8 heads x 128, bf16: 134 MB in 20.8 us, 6.4 TB/s). A warp takes one row of one side (kv_heads * head_dim values, 16 bytes of the cache per
-// lane at a time, four of them in flight), so that the slot is read and divided once per row.
+// lane at a time, four of them in flight), so that the slot is read and divided once per row. (No __restrict__: the compiler would read what the
+// kernel before this one may still be writing through the read-only path.)
 constexpr int kAppendWarps = 8;
 
 template <class Out> __device__ __forceinline__ uint32_t pack2(float a, float b, bool &bad) {
@@ -185,10 +186,9 @@ template <class In> __device__ __forceinline__ float2 unpack2(uint32_t w) {
 template <class In> struct AppendVec { uint4 w[sizeof(In) / 2]; };      // eight values of the source
 
 template <class In, class Out>
-__global__ void __launch_bounds__(32 * kAppendWarps) kv_append_kernel(const int64_t *__restrict__ slots, uint64_t tokens, const In *__restrict__ k,
-                                                                      uint64_t k_stride, const In *__restrict__ v, uint64_t v_stride,
-                                                                      uint64_t total_slots, uint32_t page_size, uint32_t kv_heads, uint32_t dim_vecs,
-                                                                      uint4 *__restrict__ k_pages, uint4 *__restrict__ v_pages, int *status) {
+__global__ void __launch_bounds__(32 * kAppendWarps) kv_append_kernel(const int64_t *slots, uint64_t tokens, const In *k, uint64_t k_stride, const In *v,
+                                                                      uint64_t v_stride, uint64_t total_slots, uint32_t page_size, uint32_t kv_heads,
+                                                                      uint32_t dim_vecs, uint4 *k_pages, uint4 *v_pages, int *status) {
     const uint64_t job = (uint64_t)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
     const uint32_t lane = threadIdx.x & 31u;
     pdl_trigger();
