@@ -8,8 +8,10 @@
 // which adds less to the output's error than its own rounding (an output of f32 would not allow that); their sum stays f32 and unrounded. f16
 // weights are lifted by 2^15 before, and their sums with them, so that those down to 2^-29 of the largest keep all their bits and smaller ones are off by at
 // most 2^-40 of it: of a million keys that is 2^-20 (unlifted, the many small weights beside one large key were lost: 2^-25 each).
-// 64 sessions of 100 to 32768 keys (3.46 GB): 558 us, 6.2 TB/s, 94 % of the copy bandwidth; equal shares of blocks instead of a fixed number of
-// slices per session are what holds that for ragged lengths. One session of 1500 keys: 12 us for the two kernels, all latency.
+// 64 sessions of 100 to 32768 keys (3.46 GB): 562 us, 6.15 TB/s, 94 % of the copy bandwidth, and 581 us (91 %) with three sets of inputs in rotation,
+// at 1740 MHz under the power cap; equal shares of blocks instead of a fixed number of slices per session are what holds that for ragged lengths.
+// One session of 1500 keys: 12 us for the two kernels, all latency. Registers: 150 to 189 with 64 dims, 168 (16 bytes spilled, 8 rows) and 248 (16 rows)
+// with 128, 255 with 256 (244 bytes spilled).
 #include <cuda_bf16.h>
 #include <float.h>
 
@@ -284,6 +286,13 @@ __global__ void __launch_bounds__(2 * D) paged_join_kernel(const PagedParams p, 
 
 // Which kernel, for how many rows a slot holds, on how many CTAs. Up to 16 rows fit the MMA of the rows kernel (8 with 256 dims, where
 // sixteen rows of Q and O would not fit the registers); beyond that its operands would be read again for every 16 rows, while a tile holds 128.
+// Device time in us of the rows kernel and of the tiles kernel for the same calls, bf16, fresh 1: 64 sessions of up to 16384 keys and 4 kv heads; 8
+// sessions of up to 4096 and 8; one of 4096 and 8:
+//   64 dims,  8 rows    77 107 |  14.9 24.6 |  18.1 15.0      128 dims,  8 rows  133 141 |  25.6 30.0 |  20.7 15.9
+//   64 dims, 16 rows   106 107 |  18.0 24.6 |  17.8 15.0      128 dims, 16 rows  147 142 |  27.2 29.6 |  20.6 15.6
+//  256 dims,  8 rows   273 249 |  48.6 42.8 |  24.0 17.2      (24 rows, tiles alone: 108, 138, 246 us of the first kind)
+// So the border holds for a few sessions and more at 64 and 128 dims (but for 3 % at 16 rows of 128 and 64 sessions); one session would gain 16 to 24 %
+// from tiles, 256 dims altogether 9 to 28 %.
 struct PagedShape { bool tiles; uint32_t rows; unsigned ctas; };
 static PagedShape paged_shape(const yvex_b200_kv_cache *c, const yvex_b200_kv_step *t, uint64_t q_heads) {
     const uint64_t group = q_heads / c->kv_heads, rows = t->longest_fresh * group, D = c->head_dim;

@@ -11,13 +11,15 @@
 // ends. 256 columns of a head leave room for one stream (O alone takes 256 of the 512 columns of tensor memory).
 //
 // The running maximum is only followed when it grows by more than kSlack powers of two: rescaling O means reading and writing it back, and a
-// weight of up to 2^kSlack costs no precision in f32 sums. f16 weights are lifted by 2^10 so that small ones do not
-// become subnormal, and follow the maximum sooner.
+// weight of up to 2^kSlack costs no precision in f32 sums. f16 weights are lifted by 2^10, so that those down to 2^-24 of the
+// maximum keep all their bits and smaller ones are off by at most 2^-35 of it, and follow the maximum sooner.
 //
-// A block of 128 keys for two tiles takes 2900 to 3100 cycles, of which the tensor cores work 2048 and the exponentials (16 a cycle and SM) as much:
-// what is left is that S and PV stand behind one another in the tensor cores' queue and that there is one buffer of S for two streams. 16 trees of
-// 32 to 64 nodes over 100 to 32768 keys (32 query heads, 8 kv heads, 128 dims, 1.02 GB of cache): 270 us, 3.8 TB/s; chunks of two prompts (573
-// GFLOP): 585 us, 0.98 PFLOP/s (307 and 592 with three sets of inputs in rotation).
+// A block of 128 keys for two tiles takes 2900 to 3000 cycles, of which the tensor cores work 2048 and the exponentials (16 a cycle and SM) as much, an
+// item 17 K besides; counted, both units are busy 58 to 61 % of an SM's active cycles. What is left is that S and PV stand behind one another
+// in the tensor cores' queue and that there is one buffer of S for two streams. 16 trees of 32 to 64 nodes over 100 to 32768 keys (32 query heads,
+// 8 kv heads, 128 dims, 1.02 GB of cache): 405 K cycles from the first CTA to the last, 349 K of them active on an SM; 256 us after a rest and 299 in a
+// row, where the power cap holds the clock at 1470 MHz (307 with three sets of inputs). Chunks of two prompts (573 GFLOP): 898 K cycles, 827 K active;
+// 522 us after a rest, 579 in a row at 1700 MHz (591 with three sets: 0.97 PFLOP/s). 168 registers at launch, 172 bytes of them spilled (64 and 128 dims).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

@@ -5,12 +5,13 @@
 // takes several rows of a request, counts its words in a hash table in shared memory (key, and one 32-bit counter: bit 31 occurs in the
 // prompt, the rest how often it was generated), and then visits the table's words for every row. Biased words enter the table first, so that they are
 // the first of its list and their last entries an array beside it (a place for them in every slot, 229 KB of shared memory in place of 160, took 24 us
-// more at 419 rows). The table is built while the
-// stream runs. Counters are integers, so the order of the atomics does not show. Requests with more words than the table holds are done in
+// more at 419 rows). With few rows the table is built while the
+// stream runs; with many the two follow one another, since an edit CTA's registers (57344 of an SM's 65536) only fit an SM that the stream has left.
+// Counters are integers, so the order of the atomics does not show. Requests with more words than the table holds are done in
 // parts of the words, halved until they fit. (One kernel with counters for a share of the vocabulary and the edits in the stream took 204 us for
 // 419 rows of 129280 words, with the edits behind the stream 175: nearly every warp meets a counted word among its 128, and every share
-// of the vocabulary counts the whole history.) Now 148: the stream 92 (435 MB, 4.7 TB/s), the edits 56. One row is 8 us of device time, two
-// launches where one kernel took 6.
+// of the vocabulary counts the whole history.) Now 148 with one set of inputs, 152 with three: the stream 92 (435 MB, 4.7 TB/s), the edits 56. One row
+// is 7.9 us of device time, two launches; as one kernel it took 6, but there is no rule yet that would choose that form for few rows.
 #include "paged.cuh"
 
 namespace yb {

@@ -27,8 +27,8 @@ struct PagedParams {
 };
 
 // What an item costs the tiles kernel besides its blocks of 128 keys (64 with 256 dims), in blocks: the first S waits for Q, the last PV is
-// waited for, the sums are read and written, and the code of all that is fetched anew. (16 trees at 100 to 32768 keys: 2 blocks 283 us,
-// 4 287, 6 253; chunks of two prompts 570, 560, 550.)
+// waited for, the sums are read and written, and the code of all that is fetched anew. (16 trees at 100 to 32768 keys with 2, 4, 6 and 8 blocks:
+// 276, 270, 265 and 268 us; chunks of two prompts 570, 565, 564 and 579; one tree 22.0, 21.8, 21.7 and 20.9: all at 128 dims, within 3 % of noise.)
 constexpr int kTilesCost = 6;
 
 // An item that a CTA began: CTAs c .. last hold its parts. rows 0: none.
