@@ -130,3 +130,15 @@ def test_scales_that_f32_cannot_carry_are_refused(L):
     for scale in (1e-40, 1.1e-38, 1e-45, 2.4e38, 3.4e38):
         assert L.lib.yvex_b200_attention_paged(cache, step, P, 1024, 8, scale, P, P, 1 << 40, P, None) == -10
     assert L.lib.yvex_b200_launch_count() == before
+
+
+def test_descriptions_filled_in_by_hand(front, monkeypatch):
+    """The structs of the C header, without what the front end remembers beside them."""
+    import torch
+    P, called = 0x10000, []
+    monkeypatch.setattr(front, "lib", N(yvex_b200_kv_plan=lambda *a: called.append(a) or 0, yvex_b200_attention_paged_workspace_bytes=lambda *a: called.append(a) or 64))
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: None)
+    step = front.KvStep(3, 12, 5, 4, 80, 0, P, P, P, P, P, P, P, P, P)
+    front.kv_plan(front.KvCache(30, 100, 16, 2, 128, P, P), step, i32(3), status(), i32(1))
+    front.attention_paged_workspace(front.KvCache(30, 100, 16, 2, 128, P, P), step, 8)
+    assert len(called) == 2

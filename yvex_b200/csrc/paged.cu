@@ -7,7 +7,7 @@ namespace yb {
 // offsets = exclusive prefix of fresh; first_page = exclusive prefix of ceil((cached + fresh) / S) - ceil(cached / S). A page
 // that a request gains starts with one of its fresh tokens (its first token has an index >= cached), so every row can be planned
 // by itself, table entry included, once the prefixes are known.
-// 64 sessions 3.6 us, 512 trees (24 K nodes) 4.8, launch included.
+// 64 sessions 3.7 us, 512 trees (24 K nodes) 4.9, launch included.
 //
 // Latency is all there is to it (a step of 64 requests moves 2 KB): one launch, and instead of a second kernel or a wait between
 // CTAs every CTA scans the lengths itself, 512 requests at a time, and keeps what concerns its own rows. Rows of a tree need their

@@ -47,21 +47,25 @@ class Mhc(C.Structure):
 
 
 class KvCache(C.Structure):
+    device = None              # whose arrays these are, where the front end has made it (None: any)
     _fields_ = [("qtype", u32), ("pages", u64), ("page_size", u64), ("kv_heads", u64), ("head_dim", u64), ("k", vp), ("v", vp)]
 
 
 class KvStep(C.Structure):
+    device = None
     _fields_ = [("requests", u64), ("tokens", u64), ("table_width", u64), ("longest_fresh", u64), ("longest", u64), ("tree", C.c_int),
                 ("cached", vp), ("fresh", vp), ("parents", vp), ("block_table", vp), ("offsets", vp), ("slots", vp), ("positions", vp),
                 ("row_request", vp), ("ancestors", vp)]
 
 
 class LogitsPolicy(C.Structure):
+    device = None
     _fields_ = [("vocabulary", u64), ("requests", u64), ("history_tokens", u64), ("bias_entries", u64), ("history", vp), ("history_offsets", vp), ("prompt_lengths", vp), ("repetition", vp),
                 ("presence", vp), ("frequency", vp), ("bias_tokens", vp), ("bias_values", vp), ("bias_offsets", vp)]
 
 
 class LogitsDrafts(C.Structure):
+    device = None
     _fields_ = [("rows", u64), ("tree", C.c_int), ("drafted", vp), ("row_request", vp), ("offsets", vp), ("ancestors", vp)]
 
 
@@ -542,26 +546,33 @@ def _need(ok, where):
         raise YvexError(INVALID_ARG, where)
 
 
+_current = []                  # torch's functions for the current device and its stream's handle, looked up once
+
+
+def _look_up():
+    torch = _torch()
+    _current[:] = (getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device,
+                   getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream))
+
+
 def _device():
     """Index of the current device, whose current stream a call goes to (the private call where torch has it: 0.4 us less)."""
-    get = getattr(_torch()._C, "_cuda_getDevice", None)
-    return get() if get else _torch().cuda.current_device()
+    if not _current:
+        _look_up()
+    return _current[0]()
 
 
 def _on(dev):
     """Raw handle of the device's current stream."""
-    torch = _torch()
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(dev) if raw else torch.cuda.current_stream(dev).cuda_stream
+    if not _current:
+        _look_up()
+    return _current[1](dev)
 
 
-def _here(dev, where, status, *described):
-    """Checks that a status word and descriptions that name arrays are of the current device; the word's address."""
-    for d in described:
-        if d.device is not None and d.device != dev:
-            raise YvexError(INVALID_ARG, where)
+def _here(dev, where, status, at, and_at=None):
+    """The address of a call's status word, which like the descriptions (`at`: their devices, None for any) is of the current device."""
     word = status.word
-    if word.get_device() != dev:
+    if word.get_device() != dev or (at != dev and at is not None) or (and_at != dev and and_at is not None):
         raise YvexError(INVALID_ARG, where)
     return word.data_ptr()
 
@@ -629,7 +640,7 @@ def kv_plan(cache, step, free_pages, status, pages_used=None):
     if pages_used is None:
         pages_used = torch.empty(1, dtype=torch.int32, device=free_pages.device)
     _check(lib.yvex_b200_kv_plan(cache, step, _array(free_pages, torch.int32, None, "kv_plan", dev), free_pages.numel(),
-                                 _array(pages_used, torch.int32, 1, "kv_plan", dev), _here(dev, "kv_plan", status, step), _on(dev)), "kv_plan")
+                                 _array(pages_used, torch.int32, 1, "kv_plan", dev), _here(dev, "kv_plan", status, step.device), _on(dev)), "kv_plan")
     step.used_tensor = pages_used
     return pages_used
 
@@ -641,13 +652,13 @@ def kv_append(cache, slots, k, v, status):
     tokens, shape = slots.numel(), k.shape
     _need(shape == v.shape and len(shape) == 3 and shape[0] == tokens and shape[1:] == cache.row and k.dtype == v.dtype and k.get_device() == v.get_device() == dev, w)
     _check(lib.yvex_b200_kv_append(cache, _array(slots, torch.int64, None, w, dev), tokens, _qtype_of(k, w), k.data_ptr(), _row_stride(k, w), v.data_ptr(),
-                                   _row_stride(v, w), _here(dev, w, status, cache), _on(dev)), w)
+                                   _row_stride(v, w), _here(dev, w, status, cache.device), _on(dev)), w)
 
 
 def attention_paged_workspace(cache, step, q_heads):
     """Scratch for attention_paged calls of this cache and step sizes."""
     torch, dev = _torch(), _device()
-    _need(cache.device == dev and step.device == dev, "attention_paged_workspace")
+    _need(cache.device in (dev, None) and step.device in (dev, None), "attention_paged_workspace")
     n = int(lib.yvex_b200_attention_paged_workspace_bytes(cache, step, q_heads))
     _need(n > 0, "attention_paged_workspace")
     return torch.empty(n, dtype=torch.uint8, device="cuda")
@@ -658,7 +669,7 @@ def attention_paged(cache, step, q, scale, status, workspace=None, out=None):
     torch, dev, w = _torch(), _device(), "attention_paged"
     shape, dtype = q.shape, q.dtype
     _need(len(shape) == 3 and shape[0] == step.rows and shape[2] == cache.row[1] and dtype == cache.dtype and q.get_device() == dev, w)
-    heads, word = shape[1], _here(dev, w, status, cache, step)
+    heads, word = shape[1], _here(dev, w, status, cache.device, step.device)
     if workspace is None:
         workspace = attention_paged_workspace(cache, step, heads)
     else:
@@ -717,7 +728,7 @@ def logits_edit(policy, drafts, logits, status, grammar=None, out=None):
         _need(grammar.dim() == 2 and grammar.shape[0] >= rows and grammar.dtype == torch.int32 and grammar.stride(1) == 1 and grammar.get_device() == dev, w)
         address, words = grammar.data_ptr(), _pitch(grammar)
     _check(lib.yvex_b200_logits_edit(policy, drafts, _qtype_of(logits, w), logits.data_ptr(), _pitch(logits), address, words, out.data_ptr(), _pitch(out),
-                                     _here(dev, w, status, policy, drafts), _on(dev)), w)
+                                     _here(dev, w, status, policy.device, drafts.device), _on(dev)), w)
     return out
 
 
