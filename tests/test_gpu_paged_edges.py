@@ -291,6 +291,32 @@ def test_attention_smallest_and_largest_scales(L, scale, fresh):  # noqa: F811
     check_attention(s, out, q, k, v, scale)
 
 
+@pytest.mark.parametrize("fresh,dim,cached", [(1, 64, 300), (1, 128, 3000), (1, 256, 300), (20, 64, 300), (20, 128, 3000), (20, 256, 300)])
+def test_attention_of_the_largest_values(L, fresh, dim, cached):  # noqa: F811
+    """Values of 65504, or its negative, throughout, and keys whose weights all round up: a mean is never more than the largest value, so it is not
+    infinite either."""
+    import torch
+    scores = np.unique(np.linspace(-0.9, -0.4, 1000).astype(np.float16))
+    weights = np.exp(scores.astype(np.float64))
+    up_most = scores[np.argsort(weights / weights.astype(np.float16).astype(np.float64))][:16]      # those that are rounded up by most
+    for few in (False, True):                                    # items split over many CTAs, and whole ones
+        s = Step(L, [cached] * (16 if few else 2), [fresh] * (16 if few else 2), 16)
+        heads = 32 if few else 1
+        _, q, k, v, cache = attend(L, s, heads, 2, dim, "float16")
+        q.zero_()
+        q[..., 0] = 1
+        k.zero_()
+        for r, x in enumerate(up_most[:len(s.cached)]):
+            k[ints(s.table[r, :up(cached + fresh, 16)]).long(), :, :, 0] = float(x)
+            k[int(s.table[r, 0]), :, 0, 0] = 0
+        v.fill_(65504)
+        v[:, :, :, dim // 2:] = -65504
+        out = torch.full_like(q, 7.0)
+        L.attention_paged(cache, s.step, q, 1.0, s.status, out=out)
+        assert s.status.read() == 0
+        check_attention(s, out, q, k, v, 1.0)
+
+
 # ---- attention: more requests than a CTA counts at a time -------------------------------------------------------------
 
 @pytest.mark.parametrize("requests,most,tree", [(127, 2, None), (128, 1, None), (129, 2, None), (300, 1, None), (1100, 2, None), (390, 20, None), (390, 40, "random"), (800, 20, "star"), (33, 140, None),

@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kRowsThreads, R == 8 && D <= 128 ? 3 : 2) page
                 a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
                 bad_out |= !isfinite(a.x) || !isfinite(a.y) || !isfinite(a.z) || !isfinite(a.w);
                 const uint64_t token = w.q.n.token + (uint32_t)row / p.group, head = (uint64_t)w.head * p.group + (uint32_t)row % p.group;
-                *reinterpret_cast<uint2 *>(p.out + (token * p.kv_heads * p.group + head) * D + d) = make_uint2(close2<T>(a.x, a.y), close2<T>(a.z, a.w));
+                *reinterpret_cast<uint2 *>(p.out + (token * p.kv_heads * p.group + head) * D + d) = make_uint2(close_means<T>(a.x, a.y), close_means<T>(a.z, a.w));
             } else {
                 if (d == 0) *reinterpret_cast<float2 *>(slot + 2 * row) = make_float2(top, sum);
                 *reinterpret_cast<float4 *>(slot + 2 * R + (d / 4 * R + row) * 4) = a;
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(2 * D) paged_join_kernel(const PagedParams p, 
     a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
     const uint32_t r = (uint32_t)(sh.first_row + row);
     const uint64_t token = (uint64_t)sh.token + r / p.group, head = (uint64_t)sh.head + r % p.group;
-    *reinterpret_cast<uint2 *>(p.out + (token * p.kv_heads * p.group + head) * D + 4 * group) = make_uint2(close2<T>(a.x, a.y), close2<T>(a.z, a.w));
+    *reinterpret_cast<uint2 *>(p.out + (token * p.kv_heads * p.group + head) * D + 4 * group) = make_uint2(close_means<T>(a.x, a.y), close_means<T>(a.z, a.w));
     if (!isfinite(a.x) || !isfinite(a.y) || !isfinite(a.z) || !isfinite(a.w)) raise(p.status, YVEX_B200_STATUS_NUMERIC);
 }
 

@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(TilePlan<D>::kThreads, 1) paged_tiles_kernel(c
                             const float y0 = __uint_as_float(a[8 * e + 2 * x]) * inv, y1 = __uint_as_float(a[8 * e + 2 * x + 1]) * inv;
                             finite = fmaf(y0, 0.0f, finite);
                             finite = fmaf(y1, 0.0f, finite);
-                            o[x] = close2<T>(y0, y1);
+                            o[x] = close_means<T>(y0, y1);
                         }
                         turn[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_uint4(o[0], o[1], o[2], o[3]);
                     }

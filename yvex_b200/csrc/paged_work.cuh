@@ -257,6 +257,15 @@ template <class T> __device__ __forceinline__ uint32_t close2(float a, float b) 
     if constexpr (std::is_same<T, __half>::value) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
     else { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
 }
+// The same of means of values. In f16, weights that were rounded up can lift a mean over the largest number, by up to 2^-11: it is no infinity.
+template <class T> __device__ __forceinline__ uint32_t close_means(float a, float b) {
+    if constexpr (std::is_same<T, __half>::value) {
+        auto within = [](float x) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x; };
+        return close2<T>(within(a), within(b));
+    } else {
+        return close2<T>(a, b);
+    }
+}
 // The words' halves that are infinities or NaN (bit 15 and 31 of the result), and the words without them.
 template <class T> __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
     constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u, one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
